@@ -1,0 +1,377 @@
+// The feed-forward operators as autograd functions: checks of arguments, what
+// is kept for the backward pass, and the backward pass itself.
+#include "ffn_ops.h"
+#include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+
+namespace ffn {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+static Tensor or_none(const c10::optional<Tensor>& t) {
+    return t.has_value() ? *t : Tensor();
+}
+
+static void check_values(const Tensor& x, const char* name) {
+    TORCH_CHECK(x.is_cuda(), name, " must be on the GPU, got ", x.device());
+    TORCH_CHECK(x.scalar_type() == at::kBFloat16 ||
+                x.scalar_type() == at::kHalf || x.scalar_type() == at::kFloat,
+                name, " must be BFloat16, Half or Float, got ",
+                x.scalar_type());
+    TORCH_CHECK(x.dim() >= 1, name, " must have at least one dimension");
+    TORCH_CHECK(x.size(-1) > 0, name, "'s last dimension must not be empty");
+    TORCH_CHECK(x.size(-1) < (1LL << 30) &&
+                x.numel() / x.size(-1) < (1LL << 30), name, " of shape ",
+                x.sizes(), " is too large");
+}
+
+static void check_same(const Tensor& x, const Tensor& t, const char* name) {
+    TORCH_CHECK(t.device() == x.device(), name, " is on ", t.device(),
+                ", x on ", x.device());
+    TORCH_CHECK(t.scalar_type() == x.scalar_type(), name, " must be ",
+                x.scalar_type(), " as x is, got ", t.scalar_type());
+}
+
+static void check_weight(const Tensor& x, const Tensor& w, long long in,
+                         const char* name) {
+    TORCH_CHECK(w.dim() == 2 && w.size(1) == in && w.size(0) > 0, name,
+                " must have shape [out, ", in, "], got ", w.sizes());
+    check_same(x, w, name);
+    // 256 rows of an operand are addressed by 32-bit byte offsets
+    TORCH_CHECK(w.size(0) <= 4000000 && in <= 4000000, name, " of shape ",
+                w.sizes(), " is too large");
+}
+
+static void check_norm_params(const Tensor& x, const Tensor& gamma,
+                              const Tensor& beta, const char* weight_name,
+                              const char* bias_name) {
+    check_params(x, gamma, x.size(-1), weight_name);
+    check_params(x, beta, x.size(-1), bias_name);
+    TORCH_CHECK(!gamma.defined() || !beta.defined() ||
+                gamma.scalar_type() == beta.scalar_type(), weight_name, " is ",
+                gamma.scalar_type(), ", ", bias_name, " ",
+                beta.scalar_type());
+}
+
+static void check_act(int64_t act) {
+    TORCH_CHECK(act >= 0 && act <= 3, "no activation ", act);
+}
+
+static bool wants_grad(const Tensor& t) {
+    return t.defined() && t.requires_grad();
+}
+
+static bool recording(std::initializer_list<Tensor> all) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor& t : all) if (wants_grad(t)) return true;
+    return false;
+}
+
+static void check_once(const char* name) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), name, " has no second derivative "
+                "(backward with create_graph=True)");
+}
+
+// Absent inputs are passed on as nothing and have no edge: bit i of the mask
+// says that input i is there, and an input's edge is found by counting.
+static int64_t present(std::initializer_list<Tensor> all) {
+    int64_t mask = 0, bit = 1;
+    for (const Tensor& t : all) {
+        if (t.defined()) mask |= bit;
+        bit <<= 1;
+    }
+    return mask;
+}
+
+static bool needs(AutogradContext* ctx, int i) {
+    const int64_t mask = ctx->saved_data["inputs"].toInt();
+    if (!(mask >> i & 1)) return false;
+    return ctx->needs_input_grad(
+        __builtin_popcountll(mask & ((1LL << i) - 1)));
+}
+
+using Maybe = c10::optional<Tensor>;
+static Maybe maybe(const Tensor& t) {
+    return t.defined() ? Maybe(t) : Maybe();
+}
+
+static Tensor contiguous_or_none(const Tensor& t) {
+    return t.defined() ? t.contiguous() : t;
+}
+
+// ---- layer norm -----------------------------------------------------------------
+struct NormFn : public torch::autograd::Function<NormFn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x,
+                          const Maybe& weight, const Maybe& bias, double eps,
+                          bool act8) {
+        const Tensor gamma = or_none(weight), beta = or_none(bias);
+        const Mat m = as_rows(x);
+        NormOut o = norm_forward(m, contiguous_or_none(gamma),
+                                 contiguous_or_none(beta), eps, true, act8,
+                                 false);
+        ctx->save_for_backward({act8 ? Tensor() : x, gamma, beta, o.mean,
+                                o.rstd, o.x8.codes, o.x8.scales});
+        ctx->saved_data["inputs"] = present({x, gamma, beta});
+        return o.y.view(x.sizes());
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        check_once("layer_norm");
+        const auto s = ctx->get_saved_variables();
+        const Tensor& dy = grads[0];
+        const at::DeviceGuard guard(dy.device());
+        const Mat d = as_rows(dy);
+        const Mat x = s[0].defined() ? as_rows(s[0]) : Mat();
+        NormGrads g = norm_backward(
+            x, {s[5], s[6]}, d, nullptr, contiguous_or_none(s[1]),
+            contiguous_or_none(s[2]), s[3], s[4], needs(ctx, 0),
+            needs(ctx, 1) || needs(ctx, 2));
+        return {g.dx.defined() ? g.dx.view(dy.sizes()) : Tensor(), g.dgamma,
+                g.dbeta, Tensor(), Tensor()};
+    }
+};
+
+Tensor layer_norm(Tensor x, c10::optional<Tensor> weight,
+                  c10::optional<Tensor> bias, double eps, bool act8) {
+    const Tensor gamma = or_none(weight), beta = or_none(bias);
+    check_values(x, "x");
+    check_norm_params(x, gamma, beta, "weight", "bias");
+    const at::DeviceGuard guard(x.device());
+    if (recording({x, gamma, beta}))
+        return NormFn::apply(x, maybe(gamma), maybe(beta), eps, act8);
+    return norm_forward(as_rows(x), contiguous_or_none(gamma),
+                        contiguous_or_none(beta), eps, false, false, false)
+        .y.view(x.sizes());
+}
+
+// ---- linear layer ----------------------------------------------------------------
+static std::vector<int64_t> out_sizes(const Tensor& x, int64_t n) {
+    std::vector<int64_t> s = x.sizes().vec();
+    s.back() = n;
+    return s;
+}
+
+struct LinearFn : public torch::autograd::Function<LinearFn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x,
+                          const Tensor& w, const Maybe& maybe_bias,
+                          const Maybe& maybe_res, int64_t act, bool act8) {
+        const Tensor bias = or_none(maybe_bias), res = or_none(maybe_res);
+        const Mat m = as_rows(x);
+        Mat r;
+        if (res.defined()) r = as_rows(res);
+        const bool through = wants_grad(x) || wants_grad(w) ||
+                             wants_grad(bias);
+        LinearOut o = linear_forward(m, as_rows(w), contiguous_or_none(bias),
+                                     res.defined() ? &r : nullptr, (int)act,
+                                     through, act8, false);
+        Packed x8;
+        if (wants_grad(w) && act8) x8 = pack(m);
+        ctx->save_for_backward({wants_grad(w) && !act8 ? x : Tensor(),
+                                wants_grad(x) ? w : Tensor(), x8.codes,
+                                x8.scales, o.u.data, o.u.scales, bias});
+        ctx->saved_data["inputs"] = present({x, w, bias, res});
+        ctx->saved_data["act"] = act;
+        ctx->saved_data["how"] = (int64_t)o.u.how;
+        return o.y.view(out_sizes(x, w.size(0)));
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        check_once("linear_act");
+        const auto s = ctx->get_saved_variables();
+        const Tensor& dy = grads[0];
+        const at::DeviceGuard guard(dy.device());
+        const bool need_x = needs(ctx, 0), need_w = needs(ctx, 1);
+        const bool need_b = needs(ctx, 2);
+        Tensor dx, dw, db;
+        if (need_x || need_w || need_b) {
+            const Kept u{s[4], s[5], (int)ctx->saved_data["how"].toInt()};
+            const int act = (int)ctx->saved_data["act"].toInt();
+            // the weight's gradient is rounded once; x unpacked from 8 bits
+            // rounds once more, and p would be the third
+            const bool act8 = need_w && s[2].defined();
+            Mat p = through_act(as_rows(dy), act, u, need_b ? s[6] : Tensor(),
+                                &db, act8);
+            if (need_w)
+                dw = weight_grad(p, as_rows(
+                    act8 ? unpack(s[2], s[3], dy.scalar_type()) : s[0]));
+            p.lo = Tensor();
+            if (need_x)
+                dx = input_grad(p, as_rows(s[1]), 0, Kept(), Tensor(), nullptr,
+                                false).t.view(out_sizes(dy, s[1].size(1)));
+        }
+        return {dx, dw, db, needs(ctx, 3) ? dy : Tensor(),
+                Tensor(), Tensor()};
+    }
+};
+
+Tensor linear_act(Tensor x, Tensor weight, c10::optional<Tensor> bias,
+                  c10::optional<Tensor> residual, int64_t act, bool act8) {
+    const Tensor b = or_none(bias), r = or_none(residual);
+    check_values(x, "x");
+    check_weight(x, weight, x.size(-1), "weight");
+    check_params(x, b, weight.size(0), "bias");
+    check_act(act);
+    if (r.defined()) {
+        check_same(x, r, "residual");
+        TORCH_CHECK(r.sizes() == at::IntArrayRef(out_sizes(x, weight.size(0))),
+                    "residual must have the output's shape ",
+                    at::IntArrayRef(out_sizes(x, weight.size(0))), ", got ",
+                    r.sizes());
+    }
+    const at::DeviceGuard guard(x.device());
+    if (recording({x, weight, b, r}))
+        return LinearFn::apply(x, weight, maybe(b), maybe(r), act, act8);
+    Mat rm;
+    if (r.defined()) rm = as_rows(r);
+    return linear_forward(as_rows(x), as_rows(weight), contiguous_or_none(b),
+                          r.defined() ? &rm : nullptr, (int)act, false, false,
+                          false)
+        .y.view(out_sizes(x, weight.size(0)));
+}
+
+// ---- the block ---------------------------------------------------------------------
+struct BlockFn : public torch::autograd::Function<BlockFn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x,
+                          const Maybe& norm_weight, const Maybe& norm_bias,
+                          const Tensor& w1, const Maybe& bias1,
+                          const Tensor& w2, const Maybe& bias2, int64_t act,
+                          double eps, bool act8) {
+        const Tensor gamma = or_none(norm_weight), beta = or_none(norm_bias);
+        const Tensor b1 = or_none(bias1), b2 = or_none(bias2);
+        const Mat m = as_rows(x);
+        NormOut n = norm_forward(m, contiguous_or_none(gamma),
+                                 contiguous_or_none(beta), eps, true, act8,
+                                 act8);
+        LinearOut a = linear_forward(as_rows(n.y), as_rows(w1),
+                                     contiguous_or_none(b1), nullptr, (int)act,
+                                     true, act8, act8);
+        LinearOut o = linear_forward(as_rows(a.y), as_rows(w2),
+                                     contiguous_or_none(b2), &m, 0, false,
+                                     false, false);
+        const Tensor none;
+        ctx->save_for_backward(
+            {act8 ? none : x, act8 ? none : n.y, act8 ? none : a.y, n.x8.codes,
+             n.x8.scales, n.y8.codes, n.y8.scales, a.y8.codes, a.y8.scales,
+             a.u.data, a.u.scales, n.mean, n.rstd, gamma, beta, w1, b1, w2,
+             b2});
+        ctx->saved_data["inputs"] = present({x, gamma, beta, w1, b1, w2, b2});
+        ctx->saved_data["act"] = act;
+        ctx->saved_data["how"] = (int64_t)a.u.how;
+        return o.y.view(x.sizes());
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        check_once("ffn_block");
+        const auto s = ctx->get_saved_variables();
+        const Tensor& dy = grads[0];
+        const at::DeviceGuard guard(dy.device());
+        const auto type = dy.scalar_type();
+        const Mat d = as_rows(dy);
+        const Tensor &w1 = s[15], &b1 = s[16], &w2 = s[17], &b2 = s[18];
+        auto need = [&](int i) { return needs(ctx, i); };
+        auto kept = [&](int plain, int packed) {
+            return as_rows(s[plain].defined()
+                ? s[plain] : unpack(s[packed], s[packed + 1], type));
+        };
+        Tensor dx, dw1, db1, dw2, db2;
+        NormGrads g;
+        if (need(5)) dw2 = weight_grad(d, kept(2, 7));
+        if (need(6)) db2 = row_sums(d, b2.scalar_type());
+        const bool norm = need(0) || need(1) || need(2);
+        const bool bias = need(4);
+        if (norm || need(3) || bias) {
+            const Kept u{s[9], s[10], (int)ctx->saved_data["how"].toInt()};
+            // The norm's gradients are sums over dh, which is rounded as it
+            // comes from the product: were p rounded before, dh would round
+            // to other values.  The weight's gradient: as in LinearFn.
+            const bool act8 = need(3) && !s[1].defined();
+            Mat p = input_grad(d, as_rows(w2),
+                               (int)ctx->saved_data["act"].toInt(), u,
+                               bias ? b1 : Tensor(), &db1, norm || act8);
+            if (norm) {
+                const Mat dh = input_grad(p, as_rows(w1), 0, Kept(), Tensor(),
+                                          nullptr, false);
+                g = norm_backward(
+                    s[0].defined() ? as_rows(s[0]) : Mat(), {s[3], s[4]},
+                    dh, &d, contiguous_or_none(s[13]),
+                    contiguous_or_none(s[14]), s[11], s[12], need(0),
+                    need(1) || need(2));
+                if (need(0)) dx = g.dx.view(dy.sizes());
+            }
+            if (!act8) p.lo = Tensor();
+            if (need(3)) dw1 = weight_grad(p, kept(1, 5));
+        }
+        return {dx, g.dgamma, g.dbeta, dw1, db1, dw2, db2, Tensor(), Tensor(),
+                Tensor()};
+    }
+};
+
+Tensor ffn_block(Tensor x, c10::optional<Tensor> norm_weight,
+                 c10::optional<Tensor> norm_bias, Tensor w1,
+                 c10::optional<Tensor> b1, Tensor w2,
+                 c10::optional<Tensor> b2, int64_t act, double eps,
+                 bool act8) {
+    const Tensor gamma = or_none(norm_weight), beta = or_none(norm_bias);
+    const Tensor c1 = or_none(b1), c2 = or_none(b2);
+    check_values(x, "x");
+    check_norm_params(x, gamma, beta, "norm_weight", "norm_bias");
+    check_weight(x, w1, x.size(-1), "w1");
+    check_weight(x, w2, w1.size(0), "w2");
+    TORCH_CHECK(w2.size(0) == x.size(-1), "w2 must have shape [", x.size(-1),
+                ", ", w1.size(0), "], got ", w2.sizes());
+    check_params(x, c1, w1.size(0), "b1");
+    check_params(x, c2, x.size(-1), "b2");
+    check_act(act);
+    const at::DeviceGuard guard(x.device());
+    if (recording({x, gamma, beta, w1, c1, w2, c2}))
+        return BlockFn::apply(x, maybe(gamma), maybe(beta), w1, maybe(c1), w2,
+                              maybe(c2), act, eps, act8);
+    const Mat m = as_rows(x);
+    const NormOut n = norm_forward(m, contiguous_or_none(gamma),
+                                   contiguous_or_none(beta), eps, false, false,
+                                   false);
+    const LinearOut a = linear_forward(as_rows(n.y), as_rows(w1),
+                                       contiguous_or_none(c1), nullptr,
+                                       (int)act, false, false, false);
+    return linear_forward(as_rows(a.y), as_rows(w2), contiguous_or_none(c2),
+                          &m, 0, false, false, false).y.view(x.sizes());
+}
+
+// ---- the 8-bit form ------------------------------------------------------------------
+std::vector<Tensor> act8_pack(Tensor x) {
+    check_values(x, "x");
+    const at::DeviceGuard guard(x.device());
+    const Packed p = pack(as_rows(x));
+    std::vector<int64_t> s = x.sizes().vec();
+    s.back() = p.scales.size(1);
+    return {p.codes.view(x.sizes()), p.scales.view(s)};
+}
+
+Tensor act8_unpack(Tensor codes, Tensor scales, int64_t type) {
+    TORCH_CHECK(codes.is_cuda() && scales.device() == codes.device(),
+                "codes and scales must be on one GPU, got ", codes.device(),
+                " and ", scales.device());
+    TORCH_CHECK(codes.scalar_type() == at::kChar &&
+                scales.scalar_type() == at::kFloat,
+                "codes must be Char and scales Float, got ",
+                codes.scalar_type(), " and ", scales.scalar_type());
+    TORCH_CHECK(codes.dim() >= 1 && codes.size(-1) > 0 &&
+                codes.size(-1) < (1LL << 30),
+                "codes of shape ", codes.sizes());
+    std::vector<int64_t> s = codes.sizes().vec();
+    const int64_t dim = s.back();
+    s.back() = (dim + 127) / 128;
+    TORCH_CHECK(scales.sizes() == at::IntArrayRef(s), "scales must have shape ",
+                at::IntArrayRef(s), ", got ", scales.sizes());
+    const at::DeviceGuard guard(codes.device());
+    const auto t = type == 0 ? at::kFloat : type == 1 ? at::kBFloat16
+                                                      : at::kHalf;
+    const int64_t rows = codes.numel() / dim;
+    return unpack(codes.contiguous().view({rows, dim}),
+                  scales.contiguous().view({rows, s.back()}), t)
+        .view(codes.sizes());
+}
+
+}  // namespace ffn

@@ -1,0 +1,176 @@
+// Shared by the feed-forward operators (layernorm.hip, linear.hip): types of
+// 16 and 32 bits behind one name, 16-byte chunks at any alignment, the
+// activations with their slopes, and the 8-bit form of an activation.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+enum Act { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_SILU = 3 };
+
+// values of a row that share one scale in the 8-bit form
+#define ACT8_GROUP 128
+// under this largest magnitude 127 / a overflows: such a group is kept as zeros
+#define ACT8_LEAST 0x1p-119f
+
+// ---- chunks of 8 values ----------------------------------------------------
+// Rows of odd length start at any multiple of the type's size; the vector
+// types below say so, and gfx950 takes such addresses in one instruction.
+template <typename T> struct Chunk;
+template <> struct Chunk<bf16_t> {
+    typedef bf16_t V __attribute__((ext_vector_type(8), aligned(2)));
+};
+template <> struct Chunk<f16_t> {
+    typedef f16_t V __attribute__((ext_vector_type(8), aligned(2)));
+};
+template <> struct Chunk<float> {
+    typedef float V __attribute__((ext_vector_type(8), aligned(4)));
+};
+typedef signed char i8x8 __attribute__((ext_vector_type(8), aligned(1)));
+
+// `left` values are there (1..8); the others read as 0 and are not written
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int left, float* v) {
+    if (left >= 8) {
+        const typename Chunk<T>::V c =
+            *reinterpret_cast<const typename Chunk<T>::V*>(p);
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)c[i];
+    } else {
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < left ? (float)p[i] : 0.0f;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int left, const float* v) {
+    if (left >= 8) {
+        typename Chunk<T>::V c;
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = (T)v[i];
+        *reinterpret_cast<typename Chunk<T>::V*>(p) = c;
+    } else {
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) if (i < left) p[i] = (T)v[i];
+    }
+}
+
+__device__ __forceinline__ void load8_codes(const signed char* p, int left,
+                                            float scale, float* v) {
+    if (left >= 8) {
+        const i8x8 c = *reinterpret_cast<const i8x8*>(p);
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)c[i] * scale;
+    } else {
+        #pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = i < left ? (float)p[i] * scale : 0.0f;
+    }
+}
+
+// ---- 8-bit form ------------------------------------------------------------
+// c = rint(x * fl(127 / a)), s = fl(a * fl(1 / 127)), a = max |x| of the
+// group.  x * fl(127 / a) is at most 127 (1 + 2^-23), so rint never leaves
+// [-127, 127].  A group with an infinity or a NaN gets s = NaN and codes 0:
+// all of it reads as NaN, so a broken activation shows in the gradients.
+struct Act8Scale { float by, scale; };
+
+__device__ __forceinline__ Act8Scale act8_scale(float a, bool finite) {
+    Act8Scale s;
+    const bool some = a >= ACT8_LEAST;
+    s.by = some && finite ? 127.0f / a : 0.0f;
+    s.scale = !finite ? __builtin_nanf("")
+                      : some ? a * (1.0f / 127.0f) : 0.0f;
+    return s;
+}
+
+// max |x| over 8 values; `finite` falls where one is an infinity or NaN
+__device__ __forceinline__ float max8(const float* v) {
+    // fmax drops NaN, so NaN is carried as an infinity
+    float a = 0.0f;
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float m = fabsf(v[i]);
+        a = fmaxf(a, m == m ? m : __builtin_inff());
+    }
+    return a;
+}
+
+__device__ __forceinline__ void store8_codes(signed char* p, int left,
+                                             const float* v, float by) {
+    i8x8 c;
+    #pragma unroll
+    for (int i = 0; i < 8; ++i)
+        // by is 0 in a group of zeros and in one that is not finite
+        c[i] = by == 0.0f ? (signed char)0
+                          : (signed char)(int)rintf(v[i] * by);
+    if (left >= 8) {
+        *reinterpret_cast<i8x8*>(p) = c;
+    } else {
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) if (i < left) p[i] = c[i];
+    }
+}
+
+// max over 16 neighbouring lanes (one group of 128 values, 8 a lane)
+__device__ __forceinline__ float max16(float a) {
+    #pragma unroll
+    for (int d = 1; d < 16; d <<= 1) a = fmaxf(a, __shfl_xor(a, d));
+    return a;
+}
+
+// ---- activations -----------------------------------------------------------
+// Phi(u), the normal distribution's integral, and phi(u) = exp(-u^2/2) /
+// sqrt(2 pi).  FAST: Abramowitz & Stegun 26.2.17 in the form of 7.1.26, one
+// exp and one reciprocal, |error| < 1.5e-7 absolute: under 2^-22, while the
+// 16-bit types it serves round to 2^-12 at best.  Otherwise erff.
+template <bool FAST>
+__device__ __forceinline__ void normal_cdf_pdf(float u, float* cdf,
+                                               float* pdf) {
+    const float e = FAST ? __expf(-0.5f * u * u) : expf(-0.5f * u * u);
+    *pdf = e * 0.3989422804014327f;
+    if (FAST) {
+        const float z = fabsf(u) * 0.7071067811865476f;
+        const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * z);
+        const float q = t * (0.254829592f + t * (-0.284496736f +
+                        t * (1.421413741f + t * (-1.453152027f +
+                        t * 1.061405429f)))) * e * 0.5f;
+        *cdf = u < 0.0f ? q : 1.0f - q;
+    } else {
+        *cdf = 0.5f * (1.0f + erff(u * 0.7071067811865476f));
+    }
+}
+
+template <bool FAST>
+__device__ __forceinline__ float act_value(float u, int act) {
+    if (act == ACT_RELU) return u > 0.0f || u != u ? u : 0.0f;
+    if (act == ACT_GELU) {
+        float cdf, pdf;
+        normal_cdf_pdf<FAST>(u, &cdf, &pdf);
+        return u * cdf;
+    }
+    if (act == ACT_SILU) return u / (1.0f + (FAST ? __expf(-u) : expf(-u)));
+    return u;
+}
+
+template <bool FAST>
+__device__ __forceinline__ float act_slope(float u, int act) {
+    if (act == ACT_GELU) {
+        float cdf, pdf;
+        normal_cdf_pdf<FAST>(u, &cdf, &pdf);
+        return cdf + u * pdf;
+    }
+    if (act == ACT_SILU) {
+        const float s = 1.0f / (1.0f + (FAST ? __expf(-u) : expf(-u)));
+        return s * (1.0f + u * (1.0f - s));
+    }
+    return 1.0f;
+}

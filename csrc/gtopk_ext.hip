@@ -737,7 +737,32 @@ std::vector<at::Tensor> bn_bwd(
     at::Tensor gamma, at::Tensor saved_mean, at::Tensor saved_rstd,
     bool relu, bool need_dz, at::Tensor stats_scratch);
 
+// feed-forward operators (ffn_autograd.hip)
+namespace ffn {
+at::Tensor layer_norm(at::Tensor x, c10::optional<at::Tensor> weight,
+                      c10::optional<at::Tensor> bias, double eps, bool act8);
+at::Tensor linear_act(at::Tensor x, at::Tensor weight,
+                      c10::optional<at::Tensor> bias,
+                      c10::optional<at::Tensor> residual, int64_t act,
+                      bool act8);
+at::Tensor ffn_block(at::Tensor x, c10::optional<at::Tensor> norm_weight,
+                     c10::optional<at::Tensor> norm_bias, at::Tensor w1,
+                     c10::optional<at::Tensor> b1, at::Tensor w2,
+                     c10::optional<at::Tensor> b2, int64_t act, double eps,
+                     bool act8);
+std::vector<at::Tensor> act8_pack(at::Tensor x);
+at::Tensor act8_unpack(at::Tensor codes, at::Tensor scales, int64_t type);
+}  // namespace ffn
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    m.def("layer_norm", &ffn::layer_norm,
+          "layer norm with its backward pass (gfx950)");
+    m.def("linear_act", &ffn::linear_act,
+          "act(x W^T + b) + residual with its backward pass (gfx950)");
+    m.def("ffn_block", &ffn::ffn_block,
+          "x + W2 act(W1 norm(x) + b1) + b2 with its backward pass (gfx950)");
+    m.def("act8_pack", &ffn::act8_pack, "8-bit form of an activation");
+    m.def("act8_unpack", &ffn::act8_unpack, "values of an 8-bit form");
     m.def("bn_fwd_train", &bn_fwd_train,
           "fused NHWC BN(+add)(+ReLU) training forward (gfx950)");
     m.def("bn_fwd_eval", &bn_fwd_eval, "fused NHWC BN eval forward");

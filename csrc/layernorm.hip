@@ -1,0 +1,281 @@
+// Layer norm forward and backward, the 8-bit form of activations, and sums
+// over rows: launches.
+#include "ffn_ops.h"
+#include <ATen/cuda/CUDAContext.h>
+#include "layernorm_kernels.h"
+
+namespace ffn {
+
+#define FFN_OK() do { hipError_t _e = hipGetLastError(); \
+    TORCH_CHECK(_e == hipSuccess, "HIP error: ", hipGetErrorString(_e)); \
+} while (0)
+
+// runs the statement with T as the tensor's type
+#define FFN_TYPES(type, ...) do { \
+    if ((type) == at::kBFloat16) { typedef bf16_t T; __VA_ARGS__; } \
+    else if ((type) == at::kHalf) { typedef f16_t T; __VA_ARGS__; } \
+    else { typedef float T; __VA_ARGS__; } \
+} while (0)
+
+static hipStream_t stream_now() {
+    return at::cuda::getCurrentCUDAStream().stream();
+}
+
+Mat as_rows(const at::Tensor& x) {
+    Mat m;
+    m.dim = x.size(-1);
+    m.rows = 1;
+    for (int64_t i = 0; i + 1 < x.dim(); ++i) m.rows *= x.size(i);
+    m.t = x.dim() == 2 ? x : x.reshape({m.rows, m.dim});
+    if (m.dim > 1 && m.t.stride(1) != 1) m.t = m.t.contiguous();
+    if (m.rows > 1 && m.t.stride(0) < m.dim) m.t = m.t.contiguous();
+    // the products address 256 rows by 32-bit byte offsets
+    if (m.rows > 1 && m.t.stride(0) > 4000000 && m.t.stride(0) != m.dim)
+        m.t = m.t.contiguous();
+    m.ld = m.rows > 1 ? m.t.stride(0) : m.dim;
+    return m;
+}
+
+void check_params(const at::Tensor& x, const at::Tensor& p, long long n,
+                  const char* name) {
+    if (!p.defined()) return;
+    TORCH_CHECK(p.dim() == 1 && p.size(0) == n, name, " must have shape [", n,
+                "], got ", p.sizes());
+    TORCH_CHECK(p.device() == x.device(), name, " is on ", p.device(),
+                ", x on ", x.device());
+    TORCH_CHECK(p.scalar_type() == x.scalar_type() ||
+                p.scalar_type() == at::kFloat, name, " must be ",
+                x.scalar_type(), " or Float, got ", p.scalar_type());
+}
+
+static long long groups_in(long long dim) {
+    return (dim + ACT8_GROUP - 1) / ACT8_GROUP;
+}
+
+Packed empty_packed(long long rows, long long dim, const at::Tensor& like) {
+    return {at::empty({rows, dim}, like.options().dtype(at::kChar)),
+            at::empty({rows, groups_in(dim)}, like.options().dtype(at::kFloat))};
+}
+
+Packed pack(const Mat& x) {
+    Packed p = empty_packed(x.rows, x.dim, x.t);
+    const long long groups = x.rows * groups_in(x.dim);
+    if (!groups) return p;
+    const int grid = (int)std::min<long long>((groups + 15) / 16, 256 * 16);
+    FFN_TYPES(x.t.scalar_type(),
+        auto k = act8_pack_kernel<T>;
+        k<<<grid, 256, 0, stream_now()>>>(
+            (const T*)x.t.data_ptr(), x.ld, x.rows, (int)x.dim,
+            (signed char*)p.codes.data_ptr(),
+            p.scales.data_ptr<float>()));
+    FFN_OK();
+    return p;
+}
+
+at::Tensor unpack(const at::Tensor& codes, const at::Tensor& scales,
+                  at::ScalarType type) {
+    const long long rows = codes.size(0), dim = codes.size(1);
+    auto out = at::empty({rows, dim}, codes.options().dtype(type));
+    const long long n = rows * ((dim + 7) / 8);
+    if (!n) return out;
+    const int grid = (int)std::min<long long>((n + 255) / 256, 256 * 16);
+    FFN_TYPES(type,
+        auto k = act8_unpack_kernel<T>;
+        k<<<grid, 256, 0, stream_now()>>>(
+            (const signed char*)codes.data_ptr(), scales.data_ptr<float>(),
+            rows, (int)dim, (T*)out.data_ptr()));
+    FFN_OK();
+    return out;
+}
+
+// team of threads a row, chunks a thread: as few threads as hold the row in 4
+// chunks each (a wave: up to 2048 values; 256 threads: 8192; 1024: 32768)
+#define NORM_SHAPES(dim, WIDE, GO) do { \
+    const long long chunks = ((dim) + 7) / 8; \
+    if (chunks <= 64) GO(64, 1); \
+    else if (chunks <= 128) GO(64, 2); \
+    else if (chunks <= 192) GO(64, 3); \
+    else if (chunks <= 256) GO(64, 4); \
+    else if (chunks <= 512) GO(256, 2); \
+    else if (chunks <= 1024) GO(256, 4); \
+    else if (chunks <= 2048) GO(1024, 2); \
+    else if (chunks <= 4096) GO(1024, 4); \
+    else WIDE; \
+} while (0)
+
+NormOut norm_forward(const Mat& x, const at::Tensor& gamma,
+                     const at::Tensor& beta, double eps, bool stats,
+                     bool keep_x8, bool keep_y8) {
+    NormOut o;
+    o.y = at::empty({x.rows, x.dim}, x.t.options());
+    const auto f32 = x.t.options().dtype(at::kFloat);
+    if (stats) {
+        o.mean = at::empty({x.rows}, f32);
+        o.rstd = at::empty({x.rows}, f32);
+    }
+    if (keep_x8) o.x8 = empty_packed(x.rows, x.dim, x.t);
+    if (keep_y8) o.y8 = empty_packed(x.rows, x.dim, x.t);
+    if (!x.rows) return o;
+    NormArgs a{};
+    a.x = x.t.data_ptr();
+    a.ld = x.ld;
+    a.gamma = gamma.defined() ? gamma.data_ptr() : nullptr;
+    a.beta = beta.defined() ? beta.data_ptr() : nullptr;
+    a.p32 = gamma.defined() ? gamma.scalar_type() == at::kFloat
+          : beta.defined() && beta.scalar_type() == at::kFloat;
+    a.y = o.y.data_ptr();
+    if (stats) {
+        a.mean = o.mean.data_ptr<float>();
+        a.rstd = o.rstd.data_ptr<float>();
+    }
+    if (keep_x8) {
+        a.x8 = (signed char*)o.x8.codes.data_ptr();
+        a.x8_scale = o.x8.scales.data_ptr<float>();
+    }
+    if (keep_y8) {
+        a.y8 = (signed char*)o.y8.codes.data_ptr();
+        a.y8_scale = o.y8.scales.data_ptr<float>();
+    }
+    a.rows = (int)x.rows;
+    a.dim = (int)x.dim;
+    a.eps = (float)eps;
+    const auto s = stream_now();
+    #define GO(NT, R) do { \
+        const int teams = NT == 64 ? 4 : 1, threads = NT == 64 ? 256 : NT; \
+        const int grid = (int)std::min<long long>( \
+            (x.rows + teams - 1) / teams, 256 * 8); \
+        auto k = norm_forward_kernel<T, NT, R>; \
+        k<<<grid, threads, 0, s>>>(a); \
+    } while (0)
+    #define WIDE do { \
+        auto k = norm_forward_wide_kernel<T>; \
+        k<<<(int)x.rows, 1024, 0, s>>>(a); \
+    } while (0)
+    FFN_TYPES(x.t.scalar_type(), NORM_SHAPES(x.dim, WIDE, GO));
+    #undef GO
+    #undef WIDE
+    FFN_OK();
+    return o;
+}
+
+static void sum_columns(const at::Tensor& part, long long n, long long width,
+                        long long first, at::Tensor a, at::Tensor b) {
+    const auto type = a.defined() ? a.scalar_type() : b.scalar_type();
+    const int grid = (int)((width + 15) / 16);
+    FFN_TYPES(type,
+        auto k = column_sum_kernel<T>;
+        k<<<grid, 1024, 0, stream_now()>>>(
+            part.data_ptr<float>(), (int)n, (int)width, (int)first,
+            a.defined() ? (T*)a.data_ptr() : nullptr,
+            b.defined() ? (T*)b.data_ptr() : nullptr));
+    FFN_OK();
+}
+
+NormGrads norm_backward(const Mat& x, const Packed& x8, const Mat& dy,
+                        const Mat* add, const at::Tensor& gamma,
+                        const at::Tensor& beta, const at::Tensor& mean,
+                        const at::Tensor& rstd, bool need_dx,
+                        bool need_params) {
+    const long long rows = dy.rows, dim = dy.dim;
+    NormGrads g;
+    if (need_dx) g.dx = at::empty({rows, dim}, dy.t.options());
+    if (need_params && gamma.defined()) g.dgamma = at::empty_like(gamma);
+    if (need_params && beta.defined()) g.dbeta = at::empty_like(beta);
+    const bool params = g.dgamma.defined() || g.dbeta.defined();
+    if (!rows) {
+        if (g.dgamma.defined()) g.dgamma.zero_();
+        if (g.dbeta.defined()) g.dbeta.zero_();
+        return g;
+    }
+    NormGradArgs a{};
+    if (x8.codes.defined()) {
+        a.x8 = (const signed char*)x8.codes.data_ptr();
+        a.x8_scale = x8.scales.data_ptr<float>();
+    } else {
+        a.x = x.t.data_ptr();
+        a.ld = x.ld;
+    }
+    a.dy = dy.t.data_ptr();
+    a.ld_dy = dy.ld;
+    if (add) {
+        a.add = add->t.data_ptr();
+        a.ld_add = add->ld;
+    }
+    a.gamma = gamma.defined() ? gamma.data_ptr() : nullptr;
+    a.p32 = gamma.defined() && gamma.scalar_type() == at::kFloat;
+    a.mean = mean.data_ptr<float>();
+    a.rstd = rstd.data_ptr<float>();
+    a.dx = need_dx ? g.dx.data_ptr() : nullptr;
+    a.rows = (int)rows;
+    a.dim = (int)dim;
+    const auto s = stream_now();
+    const auto f32 = dy.t.options().dtype(at::kFloat);
+    at::Tensor part;
+    long long blocks = 0;
+    #define GO(NT, R) do { \
+        const int teams = NT == 64 ? 4 : 1, threads = NT == 64 ? 256 : NT; \
+        blocks = std::min<long long>((rows + teams - 1) / teams, \
+                                     NT == 64 ? 768 : NT == 256 ? 512 : 256); \
+        if (params) { \
+            part = at::empty({blocks, 2, dim}, f32); \
+            a.part = part.data_ptr<float>(); \
+        } \
+        auto k = norm_backward_kernel<T, NT, R>; \
+        k<<<(int)blocks, threads, 0, s>>>(a); \
+    } while (0)
+    #define WIDE do { \
+        if (need_dx) { \
+            auto k = norm_dx_wide_kernel<T>; \
+            k<<<(int)rows, 1024, 0, s>>>(a); \
+        } \
+        if (params) { \
+            const int per = (int)std::max<long long>(64, (rows + 63) / 64); \
+            blocks = (rows + per - 1) / per; \
+            part = at::empty({blocks, 2, dim}, f32); \
+            a.part = part.data_ptr<float>(); \
+            const dim3 grid((unsigned)((dim + 255) / 256), (unsigned)blocks); \
+            auto k = row_sum_kernel<T, true>; \
+            k<<<grid, 256, 0, s>>>(a, per); \
+        } \
+    } while (0)
+    FFN_TYPES(dy.t.scalar_type(), NORM_SHAPES(dim, WIDE, GO));
+    #undef GO
+    #undef WIDE
+    FFN_OK();
+    if (params) sum_columns(part, blocks, 2 * dim, dim, g.dgamma, g.dbeta);
+    return g;
+}
+
+at::Tensor row_sums(const Mat& p, at::ScalarType type) {
+    auto out = at::empty({p.dim}, p.t.options().dtype(type));
+    if (!p.rows) return out.zero_();
+    // about 2048 blocks, of 32 rows at least
+    const long long cols = (p.dim + 255) / 256;
+    const long long slabs = std::max<long long>(1, 2048 / cols);
+    const int per = (int)std::max<long long>(32, (p.rows + slabs - 1) / slabs);
+    const long long blocks = (p.rows + per - 1) / per;
+    auto part = at::empty({blocks, p.dim}, p.t.options().dtype(at::kFloat));
+    NormGradArgs a{};
+    a.dy = p.t.data_ptr();
+    a.ld_dy = p.ld;
+    a.part = part.data_ptr<float>();
+    a.rows = (int)p.rows;
+    a.dim = (int)p.dim;
+    const dim3 grid((unsigned)cols, (unsigned)blocks);
+    FFN_TYPES(p.t.scalar_type(),
+        auto k = row_sum_kernel<T, false>;
+        k<<<grid, 256, 0, stream_now()>>>(a, per));
+    FFN_OK();
+    sum_columns(part, blocks, p.dim, p.dim, out, at::Tensor());
+    return out;
+}
+
+// sums of `n` rows of partial sums, for linear.hip
+at::Tensor sum_partials(const at::Tensor& part, long long n, long long width,
+                        at::ScalarType type) {
+    auto out = at::empty({width}, part.options().dtype(type));
+    sum_columns(part, n, width, width, out, at::Tensor());
+    return out;
+}
+
+}  // namespace ffn

@@ -1,0 +1,455 @@
+// !!! This is a file automatically generated by hipify!!!
+#include "hip/hip_runtime.h"
+// Kernels of the layer norm, of the 8-bit form of activations, and of sums
+// over rows.
+#pragma once
+#include "ffn_common.h"
+
+// ---- reductions --------------------------------------------------------------
+__device__ __forceinline__ float wave_sum(float v) {
+    #pragma unroll
+    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+    return v;
+}
+
+// sums of two values over the NT threads of a team (a wave or a block).  slot:
+// 2 * 16 floats that no thread still reads; blocks alternate between two.
+template <int NT>
+__device__ __forceinline__ void team_sum2(float& a, float& b, float* slot) {
+    a = wave_sum(a);
+    b = wave_sum(b);
+    if (NT > 64) {
+        const int w = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) { slot[w] = a; slot[16 + w] = b; }
+        __syncthreads();
+        a = b = 0.0f;
+        #pragma unroll
+        for (int i = 0; i < NT / 64; ++i) { a += slot[i]; b += slot[16 + i]; }
+    }
+}
+
+// ---- layer norm ---------------------------------------------------------------
+struct NormArgs {
+    const void* x;        // [rows, dim] of T, rows ld apart
+    long long ld;
+    const void* gamma;    // [dim] of T, or of float where p32; null: ones
+    const void* beta;     // null: zeros
+    void* y;              // [rows, dim]
+    float* mean;          // [rows], with rstd; null: not kept
+    float* rstd;
+    signed char* x8;      // 8-bit form of x, or null
+    float* x8_scale;
+    signed char* y8;      // 8-bit form of y, or null
+    float* y8_scale;
+    int rows, dim, p32;
+    float eps;
+};
+
+__device__ __forceinline__ int groups_of(int dim) {
+    return (dim + ACT8_GROUP - 1) / ACT8_GROUP;
+}
+
+template <typename T>
+__device__ __forceinline__ void load_param(const void* p, int p32, int c,
+                                           int left, float other, float* v) {
+    if (!p) {
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = other;
+    } else if (p32) {
+        load8((const float*)p + c, left, v);
+    } else {
+        load8((const T*)p + c, left, v);
+    }
+}
+
+// the 8-bit form of 8 columns from c on; 16 lanes hold a group
+__device__ __forceinline__ void keep8(signed char* codes, float* scales,
+                                      long long row, int c, int left, int dim,
+                                      const float* v) {
+    const float a = max16(max8(v));
+    const Act8Scale s = act8_scale(a, a < __builtin_inff());
+    if (left > 0) {
+        store8_codes(codes + row * dim + c, left, v, s.by);
+        if (c % ACT8_GROUP == 0)
+            scales[row * groups_of(dim) + c / ACT8_GROUP] = s.scale;
+    }
+}
+
+// From q, the sum of d^2, and `more`, that of d = x - mean, which rounding of
+// the mean leaves: the mean without it, and 1 / the deviation.  A row of one
+// value far from 0 so keeps no trace of its size.
+__device__ __forceinline__ float norm_rstd(float q, float more, float n,
+                                           float eps, float* mean) {
+    more /= n;
+    *mean += more;
+    const float var = q / n - more * more;
+    return 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + eps);
+}
+
+// A team of NT threads takes a row at a time and holds it in registers, R
+// chunks of 8 a thread: x is read once, the mean comes first and the variance
+// from what is left of it.
+template <typename T, int NT, int R>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_forward_kernel(
+        NormArgs p) {
+    constexpr int TEAMS = NT < 256 ? 256 / NT : 1;
+    __shared__ float slots[2][32];
+    const int t = threadIdx.x % NT;
+    float g[R][8], b[R][8];
+    #pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int c = (i * NT + t) * 8;
+        load_param<T>(p.gamma, p.p32, c, p.dim - c, 1.0f, g[i]);
+        load_param<T>(p.beta, p.p32, c, p.dim - c, 0.0f, b[i]);
+    }
+    const float n = p.dim;
+    for (int row = blockIdx.x * TEAMS + threadIdx.x / NT; row < p.rows;
+         row += gridDim.x * TEAMS) {
+        const T* x = (const T*)p.x + row * p.ld;
+        float v[R][8], s = 0.0f, q = 0.0f, none = 0.0f;
+        #pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int c = (i * NT + t) * 8;
+            load8(x + c, p.dim - c, v[i]);
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) s += v[i][j];
+        }
+        team_sum2<NT>(s, none, slots[0]);
+        float mean = s / n, more = 0.0f;
+        #pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int left = p.dim - (i * NT + t) * 8;
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float d = j < left ? v[i][j] - mean : 0.0f;
+                q += d * d;
+                more += d;
+            }
+        }
+        team_sum2<NT>(q, more, slots[1]);
+        const float rstd = norm_rstd(q, more, n, p.eps, &mean);
+        if (t == 0 && p.mean) { p.mean[row] = mean; p.rstd[row] = rstd; }
+        #pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int c = (i * NT + t) * 8, left = p.dim - c;
+            if (p.x8) keep8(p.x8, p.x8_scale, row, c, left, p.dim, v[i]);
+            #pragma unroll
+            for (int j = 0; j < 8; ++j)
+                v[i][j] = (v[i][j] - mean) * rstd * g[i][j] + b[i][j];
+            if (left > 0)
+                store8((T*)p.y + (long long)row * p.dim + c, left, v[i]);
+            if (p.y8) {
+                #pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    v[i][j] = j < left ? (float)(T)v[i][j] : 0.0f;
+                keep8(p.y8, p.y8_scale, row, c, left, p.dim, v[i]);
+            }
+        }
+    }
+}
+
+struct NormGradArgs {
+    const void* x;        // [rows, dim] of T, or its 8-bit form
+    long long ld;
+    const signed char* x8;
+    const float* x8_scale;
+    const void* dy;       // [rows, dim] of T, rows ld_dy apart
+    long long ld_dy;
+    const void* add;      // [rows, dim] of T that goes onto dx, or null
+    long long ld_add;
+    const void* gamma;
+    const float* mean;
+    const float* rstd;
+    void* dx;             // [rows, dim], or null
+    float* part;          // [blocks, 2, dim]: sums of dy xh, of dy; or null
+    int rows, dim, p32;
+};
+
+template <typename T>
+__device__ __forceinline__ void load_kept(const NormGradArgs& p, long long row,
+                                          int c, int left, float* v) {
+    if (p.x8)
+        load8_codes(p.x8 + row * p.dim + c, left,
+                    left > 0 ? p.x8_scale[row * groups_of(p.dim) +
+                                          c / ACT8_GROUP] : 0.0f, v);
+    else
+        load8((const T*)p.x + row * p.ld + c, left, v);
+}
+
+// dx = rstd (g dy - mean(g dy) - xh mean(g dy xh)).  x and dy are read once;
+// each thread sums dy xh and dy for its own columns over the rows that it
+// sees, the teams of a block add theirs in turn, and column_sum_kernel adds
+// the blocks': no atomics, the same result each time.
+template <typename T, int NT, int R>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_backward_kernel(
+        NormGradArgs p) {
+    constexpr int TEAMS = NT < 256 ? 256 / NT : 1;
+    __shared__ float slots[2][32];
+    __shared__ float all[TEAMS > 1 ? 2 * NT * R * 8 : 1];
+    const int t = threadIdx.x % NT, team = threadIdx.x / NT;
+    float g[R][8], sg[R][8], sb[R][8];
+    #pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int c = (i * NT + t) * 8;
+        load_param<T>(p.gamma, p.p32, c, p.dim - c, 1.0f, g[i]);
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) sg[i][j] = sb[i][j] = 0.0f;
+    }
+    const float inv = 1.0f / p.dim;
+    int turn = 0;
+    for (int row = blockIdx.x * TEAMS + team; row < p.rows;
+         row += gridDim.x * TEAMS, turn ^= 1) {
+        const float mean = p.mean[row], rstd = p.rstd[row];
+        float h[R][8], d[R][8], s1 = 0.0f, s2 = 0.0f;
+        #pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int c = (i * NT + t) * 8, left = p.dim - c;
+            load_kept<T>(p, row, c, left, h[i]);
+            load8((const T*)p.dy + row * p.ld_dy + c, left, d[i]);
+        }
+        #pragma unroll
+        for (int i = 0; i < R; ++i) {
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                // columns that are not there have dy = 0
+                h[i][j] = (h[i][j] - mean) * rstd;
+                sg[i][j] += d[i][j] * h[i][j];
+                sb[i][j] += d[i][j];
+                d[i][j] *= g[i][j];
+                s1 += d[i][j];
+                s2 += d[i][j] * h[i][j];
+            }
+        }
+        if (!p.dx) continue;
+        team_sum2<NT>(s1, s2, slots[turn]);
+        s1 *= inv;
+        s2 *= inv;
+        #pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int c = (i * NT + t) * 8, left = p.dim - c;
+            if (left <= 0) continue;
+            float a[8];
+            if (p.add) load8((const T*)p.add + row * p.ld_add + c, left, a);
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float v = rstd * (d[i][j] - s1 - h[i][j] * s2);
+                d[i][j] = p.add ? v + a[j] : v;
+            }
+            store8((T*)p.dx + (long long)row * p.dim + c, left, d[i]);
+        }
+    }
+    if (!p.part) return;
+    float* out = p.part + (long long)blockIdx.x * 2 * p.dim;
+    if (TEAMS == 1) {
+        #pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int c = (i * NT + t) * 8, left = p.dim - c;
+            if (left <= 0) continue;
+            store8(out + c, left, sg[i]);
+            store8(out + p.dim + c, left, sb[i]);
+        }
+        return;
+    }
+    for (int w = 0; w < TEAMS; ++w) {
+        if (team == w) {
+            #pragma unroll
+            for (int i = 0; i < R; ++i)
+                #pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    float* a = all + (i * 8 + j) * NT + t;
+                    a[0] = (w ? a[0] : 0.0f) + sg[i][j];
+                    a[R * 8 * NT] = (w ? a[R * 8 * NT] : 0.0f) + sb[i][j];
+                }
+        }
+        __syncthreads();
+    }
+    for (int c = threadIdx.x; c < 2 * p.dim; c += blockDim.x) {
+        const int col = c < p.dim ? c : c - p.dim;
+        const int k = col >> 3, at = ((k / NT) * 8 + (col & 7)) * NT + k % NT;
+        out[c] = all[(c < p.dim ? 0 : R * 8 * NT) + at];
+    }
+}
+
+// rows too long for a block's registers: they are read again for each step
+template <typename T>
+__global__ __launch_bounds__(1024) void norm_forward_wide_kernel(NormArgs p) {
+    __shared__ float slots[2][32];
+    const int row = blockIdx.x, step = 1024 * 8;
+    const T* x = (const T*)p.x + row * p.ld;
+    float s = 0.0f, q = 0.0f, none = 0.0f, v[8], g[8], b[8];
+    for (int c = threadIdx.x * 8; c < p.dim; c += step) {
+        load8(x + c, p.dim - c, v);
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) s += v[j];
+    }
+    team_sum2<1024>(s, none, slots[0]);
+    const float n = p.dim;
+    float mean = s / n, more = 0.0f;
+    for (int c = threadIdx.x * 8; c < p.dim; c += step) {
+        load8(x + c, p.dim - c, v);
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float d = j < p.dim - c ? v[j] - mean : 0.0f;
+            q += d * d;
+            more += d;
+        }
+    }
+    team_sum2<1024>(q, more, slots[1]);
+    const float rstd = norm_rstd(q, more, n, p.eps, &mean);
+    if (threadIdx.x == 0 && p.mean) { p.mean[row] = mean; p.rstd[row] = rstd; }
+    // whole groups of lanes go on together, for keep8
+    for (int c0 = 0; c0 < p.dim; c0 += step) {
+        const int c = c0 + threadIdx.x * 8, left = p.dim - c;
+        load8(x + c, left, v);
+        if (p.x8) keep8(p.x8, p.x8_scale, row, c, left, p.dim, v);
+        load_param<T>(p.gamma, p.p32, c, left, 1.0f, g);
+        load_param<T>(p.beta, p.p32, c, left, 0.0f, b);
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = (v[j] - mean) * rstd * g[j] + b[j];
+        if (left > 0) store8((T*)p.y + (long long)row * p.dim + c, left, v);
+        if (p.y8) {
+            #pragma unroll
+            for (int j = 0; j < 8; ++j)
+                v[j] = j < left ? (float)(T)v[j] : 0.0f;
+            keep8(p.y8, p.y8_scale, row, c, left, p.dim, v);
+        }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(1024) void norm_dx_wide_kernel(NormGradArgs p) {
+    __shared__ float slots[32];
+    const int row = blockIdx.x, step = 1024 * 8;
+    const float mean = p.mean[row], rstd = p.rstd[row];
+    float s1 = 0.0f, s2 = 0.0f, h[8], d[8], g[8], a[8];
+    for (int c = threadIdx.x * 8; c < p.dim; c += step) {
+        load_kept<T>(p, row, c, p.dim - c, h);
+        load8((const T*)p.dy + row * p.ld_dy + c, p.dim - c, d);
+        load_param<T>(p.gamma, p.p32, c, p.dim - c, 1.0f, g);
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            s1 += d[j] * g[j];
+            s2 += d[j] * g[j] * (h[j] - mean) * rstd;
+        }
+    }
+    team_sum2<1024>(s1, s2, slots);
+    s1 /= p.dim;
+    s2 /= p.dim;
+    for (int c = threadIdx.x * 8; c < p.dim; c += step) {
+        const int left = p.dim - c;
+        load_kept<T>(p, row, c, left, h);
+        load8((const T*)p.dy + row * p.ld_dy + c, left, d);
+        load_param<T>(p.gamma, p.p32, c, left, 1.0f, g);
+        if (p.add) load8((const T*)p.add + row * p.ld_add + c, left, a);
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float v = rstd * (d[j] * g[j] - s1 -
+                                    (h[j] - mean) * rstd * s2);
+            d[j] = p.add ? v + a[j] : v;
+        }
+        store8((T*)p.dx + (long long)row * p.dim + c, left, d);
+    }
+}
+
+// ---- sums over rows -------------------------------------------------------------
+// part[blockIdx.y][c] = sum over the slab's rows; 8 columns a thread.  NORM:
+// dy xh and dy of the layer norm's gradients, else the rows of p.dy alone.
+template <typename T, bool NORM>
+__global__ __launch_bounds__(256) void row_sum_kernel(NormGradArgs p,
+                                                      int per) {
+    __shared__ float all[8 * 256];
+    const int t = threadIdx.x & 31, r0 = threadIdx.x >> 5;
+    const int c = (blockIdx.x * 32 + t) * 8, left = p.dim - c;
+    const int first = blockIdx.y * per;
+    const int last = p.rows - first < per ? p.rows : first + per;
+    float sg[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sb[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (left > 0) {
+        #pragma unroll 4
+        for (int row = first + r0; row < last; row += 8) {
+            float d[8], h[8];
+            load8((const T*)p.dy + row * p.ld_dy + c, left, d);
+            if (NORM) {
+                load_kept<T>(p, row, c, left, h);
+                #pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    sg[j] += d[j] * (h[j] - p.mean[row]) * p.rstd[row];
+            }
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) sb[j] += d[j];
+        }
+    }
+    for (int half = 0; half < (NORM ? 2 : 1); ++half) {
+        #pragma unroll
+        for (int j = 0; j < 8; ++j)
+            all[r0 * 256 + t * 8 + j] = NORM && !half ? sg[j] : sb[j];
+        __syncthreads();
+        const int col = blockIdx.x * 256 + threadIdx.x;
+        float s = 0.0f;
+        for (int r = 0; r < 8; ++r) s += all[r * 256 + threadIdx.x];
+        if (col < p.dim)
+            p.part[((long long)blockIdx.y * (NORM ? 2 : 1) + half) * p.dim +
+                   col] = s;
+        __syncthreads();
+    }
+}
+
+// out[c] = sum over `n` rows of part, width values each, in a fixed order; the
+// first `first` columns go to `a`, the others to `b` (either may be null)
+template <typename O>
+__global__ __launch_bounds__(1024) void column_sum_kernel(
+        const float* part, int n, int width, int first, O* a, O* b) {
+    __shared__ float all[64][17];
+    const int t = threadIdx.x & 15, r0 = threadIdx.x >> 4;
+    const int c = blockIdx.x * 16 + t;
+    float s = 0.0f;
+    if (c < width) {
+        #pragma unroll 4
+        for (int r = r0; r < n; r += 64) s += part[(long long)r * width + c];
+    }
+    all[r0][t] = s;
+    __syncthreads();
+    if (threadIdx.x < 16 && c < width) {
+        float v = 0.0f;
+        #pragma unroll 8
+        for (int r = 0; r < 64; ++r) v += all[r][t];
+        if (c < first) { if (a) a[c] = (O)v; }
+        else if (b) b[c - first] = (O)v;
+    }
+}
+
+// ---- the 8-bit form by itself ------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(256) void act8_pack_kernel(
+        const T* x, long long ld, long long rows, int dim, signed char* codes,
+        float* scales) {
+    const int ng = groups_of(dim);
+    const long long groups = rows * ng, step = (long long)gridDim.x * 16;
+    // all lanes of a wave go round as often, for max16
+    for (long long g0 = (long long)blockIdx.x * 16; g0 < groups; g0 += step) {
+        const long long g = g0 + (threadIdx.x >> 4);
+        const bool on = g < groups;
+        const long long row = on ? g / ng : 0;
+        const int c = (int)(g - row * ng) * ACT8_GROUP + (threadIdx.x & 15) * 8;
+        const int left = on ? dim - c : 0;
+        float v[8];
+        load8(x + row * ld + c, left, v);
+        keep8(codes, scales, row, c, left, dim, v);
+    }
+}
+
+template <typename O>
+__global__ __launch_bounds__(256) void act8_unpack_kernel(
+        const signed char* codes, const float* scales, long long rows, int dim,
+        O* out) {
+    const int nc = (dim + 7) / 8;
+    const long long n = rows * nc, step = (long long)gridDim.x * 256;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n;
+         i += step) {
+        const long long row = i / nc;
+        const int c = (int)(i - row * nc) * 8;
+        float v[8];
+        load8_codes(codes + row * dim + c, dim - c,
+                    scales[row * groups_of(dim) + c / ACT8_GROUP], v);
+        store8(out + row * dim + c, dim - c, v);
+    }
+}

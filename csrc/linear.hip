@@ -1,0 +1,278 @@
+// Products of linear layers: choice of tile and of the split over k, launches.
+#include "ffn_ops.h"
+#include <ATen/cuda/CUDAContext.h>
+#include "linear_kernels.h"
+
+namespace ffn {
+
+#define FFN_OK() do { hipError_t _e = hipGetLastError(); \
+    TORCH_CHECK(_e == hipSuccess, "HIP error: ", hipGetErrorString(_e)); \
+} while (0)
+
+#define FFN_TYPES(type, ...) do { \
+    if ((type) == at::kBFloat16) { typedef bf16_t T; __VA_ARGS__; } \
+    else if ((type) == at::kHalf) { typedef f16_t T; __VA_ARGS__; } \
+    else { typedef float T; __VA_ARGS__; } \
+} while (0)
+
+at::Tensor sum_partials(const at::Tensor& part, long long n, long long width,
+                        at::ScalarType type);
+
+static hipStream_t stream_now() {
+    return at::cuda::getCurrentCUDAStream().stream();
+}
+
+struct Plan { int tile, splits; };
+
+// Estimated time in us of the product with each tile and split, the least one
+// wins.  A tile's step over 128 bytes of k takes `step` us while `at_once`
+// blocks share a compute unit; `over` is what a block spends outside its loop.
+static Plan plan_product(long long M, long long N, long long K, int size,
+                         bool quantises) {
+    struct Shape { int tile, at_once; float step, over; };
+    static const Shape half[] = {{256, 1, 1.75f, 6.0f}, {128, 2, 1.0f, 4.0f},
+                                 {64, 5, 0.8f, 3.0f}};
+    static const Shape full[] = {{128, 2, 4.0f, 5.0f}, {64, 5, 2.6f, 3.0f}};
+    const Shape* shapes = size == 2 ? half : full;
+    const int n = size == 2 ? 3 : 2;
+    const long long steps = (K * size + 127) / 128;
+    Plan best{shapes[0].tile, 1};
+    float least = 1e30f;
+    for (int i = 0; i < n; ++i) {
+        const Shape& s = shapes[i];
+        if (quantises && s.tile < ACT8_GROUP) continue;
+        const long long tiles = ((M + s.tile - 1) / s.tile) *
+                                ((N + s.tile - 1) / s.tile);
+        for (int splits = 1; splits <= 16 && splits <= steps; ++splits) {
+            const long long per = (steps + splits - 1) / splits;
+            const long long parts = (steps + per - 1) / per;
+            if (parts != splits) continue;
+            const long long all = tiles * splits;
+            const long long slots = 256LL * s.at_once;
+            const long long rounds = (all + slots - 1) / slots;
+            // a last round that is not full runs with fewer blocks a unit
+            float t = rounds * (per * s.step + s.over);
+            if (all < slots) {
+                const float share = (float)((all + 255) / 256) / s.at_once;
+                t = per * s.step * (0.5f + 0.5f * share) + s.over;
+            }
+            if (splits > 1)
+                t += 4.0f + (float)M * N * 4.0f * (2 * splits) / 4.0e6f;
+            if (t < least) { least = t; best = {s.tile, splits}; }
+        }
+    }
+    return best;
+}
+
+template <typename T, int BM, int BN, int WM, int WN, bool AA, bool BA,
+          int EPI>
+static void launch(const Operand& a, const Operand& b, int M, int N, int K,
+                   int splits, EpiArgs e, const at::Tensor& like,
+                   long long* blocks) {
+    typedef Gemm<T, BM, BN, WM, WN, AA, BA> G;
+    const auto s = stream_now();
+    const long long tm = (M + BM - 1) / BM, tn = (N + BN - 1) / BN;
+    TORCH_CHECK(tm * tn < (1LL << 31), "product of ", M, " x ", N,
+                " is too large");
+    const int steps = (K + G::BK - 1) / G::BK;
+    const int per = (steps + splits - 1) / splits;
+    const int parts = (steps + per - 1) / per;
+    const long long ld_part = (N + 3) / 4 * 4;
+    at::Tensor part;
+    if (parts > 1)
+        part = at::empty({parts, M, ld_part},
+                         like.options().dtype(at::kFloat));
+    float* pp = parts > 1 ? part.data_ptr<float>() : nullptr;
+    const dim3 grid((unsigned)(tm * tn), (unsigned)parts);
+    auto k = gemm_kernel<T, BM, BN, WM, WN, AA, BA, EPI>;
+    k<<<grid, G::THREADS, G::LDS, s>>>(a, b, M, N, K, per * G::BK, pp,
+                                       ld_part, e);
+    FFN_OK();
+    *blocks = tm;
+    if (parts > 1) {
+        const dim3 fgrid((unsigned)((M + FINISH_ROWS - 1) / FINISH_ROWS),
+                         (unsigned)((N + 127) / 128));
+        auto f = finish_kernel<T, EPI, float>;
+        f<<<fgrid, 256, 0, s>>>(pp, ld_part, parts, M, N, e);
+        FFN_OK();
+        *blocks = fgrid.x;
+    }
+}
+
+// C = A B with the epilogue; `blocks`: rows of e.colsum that were written
+template <bool AA, bool BA, int EPI>
+static void product(at::ScalarType type, const Operand& a, const Operand& b,
+                    long long M, long long N, long long K, EpiArgs e,
+                    const at::Tensor& like, long long* blocks) {
+    const bool quantises = e.out8 || e.keep == KEEP_8BIT;
+    const Plan p = plan_product(M, N, a.lo ? 2 * K : K, type == at::kFloat ? 4 : 2,
+                                EPI == EPI_FORWARD && quantises);
+    FFN_TYPES(type,
+        if (p.tile == 256) {
+            if constexpr (sizeof(T) == 2)
+                launch<T, 256, 256, 2, 4, AA, BA, EPI>(
+                    a, b, (int)M, (int)N, (int)K, p.splits, e, like, blocks);
+        } else if (p.tile == 128) {
+            launch<T, 128, 128, 2, 2, AA, BA, EPI>(
+                a, b, (int)M, (int)N, (int)K, p.splits, e, like, blocks);
+        } else {
+            launch<T, 64, 64, 2, 2, AA, BA, EPI>(
+                a, b, (int)M, (int)N, (int)K, p.splits, e, like, blocks);
+        });
+}
+
+static Operand operand(const Mat& m) {
+    return {m.t.data_ptr(), m.ld, m.lo.defined() ? m.lo.data_ptr() : nullptr};
+}
+
+static Kept empty_kept(int act, bool act8, long long rows, long long dim,
+                       const at::Tensor& like) {
+    Kept u;
+    if (act == ACT_RELU) {
+        u.how = KEEP_BITS;
+        u.data = at::empty({rows, (dim + 7) / 8},
+                           like.options().dtype(at::kByte));
+    } else if (act != ACT_NONE && act8) {
+        Packed p = empty_packed(rows, dim, like);
+        u.how = KEEP_8BIT;
+        u.data = p.codes;
+        u.scales = p.scales;
+    } else if (act != ACT_NONE) {
+        u.how = KEEP_FULL;
+        u.data = at::empty({rows, dim}, like.options());
+    }
+    return u;
+}
+
+static void set_kept(EpiArgs& e, const Kept& u) {
+    e.keep = u.how;
+    e.kept = u.data.defined() ? u.data.data_ptr() : nullptr;
+    e.kept_scale = u.scales.defined() ? u.scales.data_ptr<float>() : nullptr;
+}
+
+LinearOut linear_forward(const Mat& x, const Mat& w, const at::Tensor& bias,
+                         const Mat* res, int act, bool keep, bool act8,
+                         bool keep_y8) {
+    LinearOut o;
+    const long long M = x.rows, N = w.rows;
+    o.y = at::empty({M, N}, x.t.options());
+    if (keep) o.u = empty_kept(act, act8, M, N, x.t);
+    if (keep_y8) o.y8 = empty_packed(M, N, x.t);
+    if (!M) return o;
+    EpiArgs e{};
+    e.out = o.y.data_ptr();
+    e.ld_out = N;
+    if (bias.defined()) {
+        e.bias = bias.data_ptr();
+        e.bias_f32 = bias.scalar_type() == at::kFloat;
+    }
+    if (res) {
+        e.res = res->t.data_ptr();
+        e.ld_res = res->ld;
+    }
+    set_kept(e, o.u);
+    if (keep_y8) {
+        e.out8 = (signed char*)o.y8.codes.data_ptr();
+        e.out8_scale = o.y8.scales.data_ptr<float>();
+    }
+    e.act = act;
+    long long blocks;
+    product<true, true, EPI_FORWARD>(x.t.scalar_type(), operand(x), operand(w),
+                                     M, N, x.dim, e, x.t, &blocks);
+    return o;
+}
+
+// rows of partial sums that any tile may write
+static at::Tensor empty_colsum(long long rows, long long dim,
+                               const at::Tensor& like) {
+    return at::empty({(rows + FINISH_ROWS - 1) / FINISH_ROWS, dim},
+                     like.options().dtype(at::kFloat));
+}
+
+static Mat empty_grad(long long rows, long long dim, const at::Tensor& like,
+                      bool split, const Kept& u) {
+    Mat p;
+    p.t = at::empty({rows, dim}, like.options());
+    // through relu a value passes whole; fp32 rounds as the sums themselves do
+    if (split && (u.how == KEEP_FULL || u.how == KEEP_8BIT) &&
+        like.scalar_type() != at::kFloat)
+        p.lo = at::empty({rows, dim}, like.options());
+    p.rows = rows;
+    p.dim = p.ld = dim;
+    return p;
+}
+
+Mat through_act(const Mat& dy, int act, const Kept& u, const at::Tensor& bias,
+                at::Tensor* dbias, bool split) {
+    if (act == ACT_NONE) {
+        if (bias.defined()) *dbias = row_sums(dy, bias.scalar_type());
+        return dy;
+    }
+    Mat p = empty_grad(dy.rows, dy.dim, dy.t, split, u);
+    if (!p.rows) {
+        if (bias.defined()) *dbias = at::zeros_like(bias);
+        return p;
+    }
+    EpiArgs e{};
+    e.out = p.t.data_ptr();
+    e.out_lo = p.lo.defined() ? p.lo.data_ptr() : nullptr;
+    e.ld_out = p.ld;
+    e.act = act;
+    set_kept(e, u);
+    at::Tensor part;
+    if (bias.defined()) {
+        part = empty_colsum(p.rows, p.dim, p.t);
+        e.colsum = part.data_ptr<float>();
+    }
+    const dim3 grid((unsigned)((p.rows + FINISH_ROWS - 1) / FINISH_ROWS),
+                    (unsigned)((p.dim + 127) / 128));
+    FFN_TYPES(dy.t.scalar_type(),
+        auto f = finish_kernel<T, EPI_GRAD, T>;
+        f<<<grid, 256, 0, stream_now()>>>((const T*)dy.t.data_ptr(), dy.ld, 1,
+                                          (int)p.rows, (int)p.dim, e));
+    FFN_OK();
+    if (bias.defined())
+        *dbias = sum_partials(part, grid.x, p.dim, bias.scalar_type());
+    return p;
+}
+
+Mat input_grad(const Mat& p, const Mat& w, int act, const Kept& u,
+               const at::Tensor& bias, at::Tensor* dbias, bool split) {
+    const long long M = p.rows, N = w.dim;
+    Mat out = empty_grad(M, N, p.t, split, u);
+    if (!M) {
+        if (bias.defined()) *dbias = at::zeros_like(bias);
+        return out;
+    }
+    EpiArgs e{};
+    e.out = out.t.data_ptr();
+    e.out_lo = out.lo.defined() ? out.lo.data_ptr() : nullptr;
+    e.ld_out = N;
+    e.act = act;
+    set_kept(e, u);
+    at::Tensor part;
+    if (bias.defined()) {
+        part = empty_colsum(M, N, p.t);
+        e.colsum = part.data_ptr<float>();
+    }
+    long long blocks;
+    product<true, false, EPI_GRAD>(p.t.scalar_type(), operand(p), operand(w),
+                                   M, N, p.dim, e, p.t, &blocks);
+    if (bias.defined())
+        *dbias = sum_partials(part, blocks, N, bias.scalar_type());
+    return out;
+}
+
+at::Tensor weight_grad(const Mat& p, const Mat& x) {
+    auto out = at::empty({p.dim, x.dim}, p.t.options());
+    if (!p.rows) return out.zero_();
+    EpiArgs e{};
+    e.out = out.data_ptr();
+    e.ld_out = x.dim;
+    long long blocks;
+    product<false, false, EPI_PLAIN>(p.t.scalar_type(), operand(p), operand(x),
+                                     p.dim, x.dim, p.rows, e, p.t, &blocks);
+    return out;
+}
+
+}  // namespace ffn

@@ -32,3 +32,7 @@ from .parallel.allreducer import (  # noqa: F401
     dense_allreduce,
 )
 from .ops.fusedbn import FusedBNAct  # noqa: F401
+from .ops.act8 import Act8, act8_pack, act8_unpack  # noqa: F401
+from .ops.ffn import FFNBlock, ffn_block  # noqa: F401
+from .ops.layernorm import FusedLayerNorm, layer_norm  # noqa: F401
+from .ops.linear import FusedLinearAct, linear_act  # noqa: F401

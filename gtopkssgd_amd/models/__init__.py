@@ -21,7 +21,8 @@ _FACTORY = {
     "resnet50": lambda num_classes=1000: resnet50(num_classes),
     "resnet101": lambda num_classes=1000: resnet101(num_classes),
     "alexnet": lambda num_classes=1000: alexnet(num_classes),
-    "lstm": lambda vocab_size=10000, hidden=1500: lstm_ptb(vocab_size, hidden),
+    "lstm": lambda vocab_size=10000, hidden=1500, ffn_mult=0, act8=False:
+        lstm_ptb(vocab_size, hidden, ffn_mult, act8),
     "lstman4": lambda hidden=512: deepspeech_an4(hidden),
 }
 

@@ -10,6 +10,8 @@ from typing import Tuple
 import torch
 import torch.nn as nn
 
+from ..ops.ffn import FFNBlock
+
 
 def repackage_hidden(h):
     """Detach hidden state from the graph (truncated BPTT)."""
@@ -21,8 +23,15 @@ def repackage_hidden(h):
 class LSTMModel(nn.Module):
     def __init__(self, vocab_size: int = 10000, emb_size: int = 1500,
                  hidden_size: int = 1500, num_layers: int = 2,
-                 dropout: float = 0.65, tie_weights: bool = True):
+                 dropout: float = 0.65, tie_weights: bool = True,
+                 ffn_mult: int = 0, act8: bool = False):
+        """ffn_mult > 0 puts a pre-norm feed-forward block of that many times
+        the hidden size between the LSTM and the decoder; act8 keeps its
+        activations in 8 bits for the backward pass."""
         super().__init__()
+        if ffn_mult < 0 or (act8 and not ffn_mult):
+            raise ValueError(f"ffn_mult={ffn_mult}, act8={act8}: act8 needs a "
+                             "feed-forward block (ffn_mult > 0)")
         self.drop = nn.Dropout(dropout)
         self.encoder = nn.Embedding(vocab_size, emb_size)
         self.rnn = nn.LSTM(emb_size, hidden_size, num_layers,
@@ -37,6 +46,8 @@ class LSTMModel(nn.Module):
         init = 0.1
         nn.init.uniform_(self.encoder.weight, -init, init)
         nn.init.zeros_(self.decoder.bias)
+        self.ffn = FFNBlock(hidden_size, ffn_mult * hidden_size, act8=act8) \
+            if ffn_mult else None
 
     def init_hidden(self, batch_size: int, device=None
                     ) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -48,11 +59,13 @@ class LSTMModel(nn.Module):
         # tokens: [seq_len, batch]
         emb = self.drop(self.encoder(tokens))
         out, hidden = self.rnn(emb, hidden)
+        if self.ffn is not None:
+            out = self.ffn(out)
         out = self.drop(out)
         logits = self.decoder(out)  # [seq, batch, vocab]
         return logits, hidden
 
 
-def lstm_ptb(vocab_size=10000, hidden=1500):
+def lstm_ptb(vocab_size=10000, hidden=1500, ffn_mult=0, act8=False):
     return LSTMModel(vocab_size=vocab_size, emb_size=hidden,
-                     hidden_size=hidden)
+                     hidden_size=hidden, ffn_mult=ffn_mult, act8=act8)

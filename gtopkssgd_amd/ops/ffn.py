@@ -1,0 +1,69 @@
+"""The pre-norm feed-forward block, one autograd function over the layer norm,
+the two products and the 8-bit form:
+
+    y = x + W2 act(W1 norm(x) + b1) + b2
+
+What goes from one operator to the next, in both directions, has x's type.  The
+backward pass takes the gradient through the activation in the epilogue of the
+product that makes it, and adds dy onto the norm's gradient in the norm's own
+pass.  With ``act8=True`` the inputs of the norm and of both products and the
+value before the activation are kept in 8 bits.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+import torch.nn as nn
+
+from . import _ext
+from .layernorm import FusedLayerNorm, layer_norm
+from .linear import _act_code, linear_act
+
+
+def ffn_block(x: torch.Tensor, norm_weight: Optional[torch.Tensor],
+              norm_bias: Optional[torch.Tensor], w1: torch.Tensor,
+              b1: Optional[torch.Tensor], w2: torch.Tensor,
+              b2: Optional[torch.Tensor], act: str = "gelu",
+              eps: float = 1e-5, act8: bool = False) -> torch.Tensor:
+    """``x + w2 act(w1 norm(x) + b1) + b2``.
+
+    x: [..., dim], w1: [hidden, dim], w2: [dim, hidden], of one type (bf16,
+    fp16 or fp32); norm_weight, norm_bias: [dim], b1: [hidden], b2: [dim], of
+    that type or fp32, or None.  Under autocast x, w1 and w2 are cast to its
+    type.  No second derivative."""
+    code = _act_code(act)
+    if x.is_cuda:
+        if torch.is_autocast_enabled("cuda"):
+            t = torch.get_autocast_dtype("cuda")
+            x, w1, w2 = x.to(t), w1.to(t), w2.to(t)
+            norm_weight, norm_bias, b1, b2 = (
+                p if p is None or p.dtype == torch.float32 else p.to(t)
+                for p in (norm_weight, norm_bias, b1, b2))
+        return _ext().ffn_block(x, norm_weight, norm_bias, w1, b1, w2, b2,
+                                code, float(eps), bool(act8))
+    if w1.dim() != 2 or w2.dim() != 2 or w2.size(0) != x.size(-1):
+        raise RuntimeError(f"w2 must have shape [{x.size(-1)}, hidden], got "
+                           f"{list(w2.shape)}")
+    h = layer_norm(x, norm_weight, norm_bias, eps, act8)
+    a = linear_act(h, w1, b1, act=act, act8=act8)
+    return linear_act(a, w2, b2, residual=x, act8=act8)
+
+
+class FFNBlock(nn.Module):
+    """``ffn_block`` with its parameters."""
+
+    def __init__(self, dim: int, hidden: int, act: str = "gelu",
+                 act8: bool = False, eps: float = 1e-5):
+        super().__init__()
+        _act_code(act)
+        self.norm = FusedLayerNorm(dim, eps=eps, act8=act8)
+        self.fc1 = nn.Linear(dim, hidden)
+        self.fc2 = nn.Linear(hidden, dim)
+        self.act = act
+        self.act8 = act8
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return ffn_block(x, self.norm.weight, self.norm.bias, self.fc1.weight,
+                         self.fc1.bias, self.fc2.weight, self.fc2.bias,
+                         self.act, self.norm.eps, self.act8)

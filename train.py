@@ -53,6 +53,12 @@ def parse_args():
     p.add_argument("--device", default=None)
     p.add_argument("--no-amp", action="store_true")
     p.add_argument("--norm-clip", type=float, default=None)
+    p.add_argument("--ffn-mult", type=int, default=0,
+                   help="lstm: pre-norm feed-forward block of this many times "
+                        "the hidden size before the decoder (0 = none)")
+    p.add_argument("--act8", action="store_true",
+                   help="lstm: keep the feed-forward block's activations in "
+                        "8 bits for the backward pass (needs --ffn-mult)")
     p.add_argument("--checkpoint-dir", default="./checkpoints")
     p.add_argument("--run-tag", default=None)
     p.add_argument("--resume", action="store_true",
@@ -66,7 +72,12 @@ def parse_args():
     p.add_argument("--torch-profile", default=None, metavar="DIR",
                    help="capture a torch.profiler chrome trace of a few "
                         "steps into DIR (rank 0)")
-    return p.parse_args()
+    args = p.parse_args()
+    if (args.ffn_mult or args.act8) and args.dnn != "lstm":
+        p.error("--ffn-mult and --act8 belong to --dnn lstm")
+    if args.ffn_mult < 0 or (args.act8 and not args.ffn_mult):
+        p.error("--act8 needs --ffn-mult of 1 or more")
+    return args
 
 
 def init_dist(args):
@@ -93,13 +104,16 @@ def main():
         f"rho{args.density}-{args.compression}-n{world}")
     metrics = JsonlLogger(args.metrics) if args.metrics and rank == 0 else None
 
+    model_kwargs = {"ffn_mult": args.ffn_mult, "act8": args.act8} \
+        if args.ffn_mult else None
     trainer = DLTrainer(
         rank=rank, size=world, dnn=args.dnn, dataset=args.dataset,
         batch_size=args.batch_size, nsteps_update=args.nsteps_update,
         lr=args.lr, device=args.device, amp=not args.no_amp,
         num_workers=args.num_workers, n_samples=args.n_samples,
         seed=args.seed, norm_clip=args.norm_clip,
-        momentum=args.momentum, weight_decay=args.weight_decay)
+        momentum=args.momentum, weight_decay=args.weight_decay,
+        model_kwargs=model_kwargs)
 
     compressor = gt.compressors[args.compression](args.density) \
         if args.compression != "none" else gt.compressors["none"]()
