@@ -1,7 +1,8 @@
 // Layer norm forward and backward, the 8-bit form of activations, and sums
 // over rows: launches.
+#include <hip/hip_runtime.h>
 #include "ffn_ops.h"
-#include <ATen/cuda/CUDAContext.h>
+#include <c10/hip/HIPStream.h>
 #include "layernorm_kernels.h"
 
 namespace ffn {
@@ -18,7 +19,7 @@ namespace ffn {
 } while (0)
 
 static hipStream_t stream_now() {
-    return at::cuda::getCurrentCUDAStream().stream();
+    return c10::hip::getCurrentHIPStream().stream();
 }
 
 Mat as_rows(const at::Tensor& x) {
@@ -64,8 +65,7 @@ Packed pack(const Mat& x) {
     const int grid = (int)std::min<long long>((groups + 15) / 16, 256 * 16);
     FFN_TYPES(x.t.scalar_type(),
         auto k = act8_pack_kernel<T>;
-        k<<<grid, 256, 0, stream_now()>>>(
-            (const T*)x.t.data_ptr(), x.ld, x.rows, (int)x.dim,
+        hipLaunchKernelGGL(k, grid, 256, 0, stream_now(), (const T*)x.t.data_ptr(), x.ld, x.rows, (int)x.dim,
             (signed char*)p.codes.data_ptr(),
             p.scales.data_ptr<float>()));
     FFN_OK();
@@ -81,8 +81,7 @@ at::Tensor unpack(const at::Tensor& codes, const at::Tensor& scales,
     const int grid = (int)std::min<long long>((n + 255) / 256, 256 * 16);
     FFN_TYPES(type,
         auto k = act8_unpack_kernel<T>;
-        k<<<grid, 256, 0, stream_now()>>>(
-            (const signed char*)codes.data_ptr(), scales.data_ptr<float>(),
+        hipLaunchKernelGGL(k, grid, 256, 0, stream_now(), (const signed char*)codes.data_ptr(), scales.data_ptr<float>(),
             rows, (int)dim, (T*)out.data_ptr()));
     FFN_OK();
     return out;
@@ -145,11 +144,11 @@ NormOut norm_forward(const Mat& x, const at::Tensor& gamma,
         const int grid = (int)std::min<long long>( \
             (x.rows + teams - 1) / teams, 256 * 8); \
         auto k = norm_forward_kernel<T, NT, R>; \
-        k<<<grid, threads, 0, s>>>(a); \
+        hipLaunchKernelGGL(k, grid, threads, 0, s, a); \
     } while (0)
     #define WIDE do { \
         auto k = norm_forward_wide_kernel<T>; \
-        k<<<(int)x.rows, 1024, 0, s>>>(a); \
+        hipLaunchKernelGGL(k, (int)x.rows, 1024, 0, s, a); \
     } while (0)
     FFN_TYPES(x.t.scalar_type(), NORM_SHAPES(x.dim, WIDE, GO));
     #undef GO
@@ -164,8 +163,7 @@ static void sum_columns(const at::Tensor& part, long long n, long long width,
     const int grid = (int)((width + 15) / 16);
     FFN_TYPES(type,
         auto k = column_sum_kernel<T>;
-        k<<<grid, 1024, 0, stream_now()>>>(
-            part.data_ptr<float>(), (int)n, (int)width, (int)first,
+        hipLaunchKernelGGL(k, grid, 1024, 0, stream_now(), part.data_ptr<float>(), (int)n, (int)width, (int)first,
             a.defined() ? (T*)a.data_ptr() : nullptr,
             b.defined() ? (T*)b.data_ptr() : nullptr));
     FFN_OK();
@@ -221,12 +219,12 @@ NormGrads norm_backward(const Mat& x, const Packed& x8, const Mat& dy,
             a.part = part.data_ptr<float>(); \
         } \
         auto k = norm_backward_kernel<T, NT, R>; \
-        k<<<(int)blocks, threads, 0, s>>>(a); \
+        hipLaunchKernelGGL(k, (int)blocks, threads, 0, s, a); \
     } while (0)
     #define WIDE do { \
         if (need_dx) { \
             auto k = norm_dx_wide_kernel<T>; \
-            k<<<(int)rows, 1024, 0, s>>>(a); \
+            hipLaunchKernelGGL(k, (int)rows, 1024, 0, s, a); \
         } \
         if (params) { \
             const int per = (int)std::max<long long>(64, (rows + 63) / 64); \
@@ -235,7 +233,7 @@ NormGrads norm_backward(const Mat& x, const Packed& x8, const Mat& dy,
             a.part = part.data_ptr<float>(); \
             const dim3 grid((unsigned)((dim + 255) / 256), (unsigned)blocks); \
             auto k = row_sum_kernel<T, true>; \
-            k<<<grid, 256, 0, s>>>(a, per); \
+            hipLaunchKernelGGL(k, grid, 256, 0, s, a, per); \
         } \
     } while (0)
     FFN_TYPES(dy.t.scalar_type(), NORM_SHAPES(dim, WIDE, GO));
@@ -264,7 +262,7 @@ at::Tensor row_sums(const Mat& p, at::ScalarType type) {
     const dim3 grid((unsigned)cols, (unsigned)blocks);
     FFN_TYPES(p.t.scalar_type(),
         auto k = row_sum_kernel<T, false>;
-        k<<<grid, 256, 0, stream_now()>>>(a, per));
+        hipLaunchKernelGGL(k, grid, 256, 0, stream_now(), a, per));
     FFN_OK();
     sum_columns(part, blocks, p.dim, p.dim, out, at::Tensor());
     return out;

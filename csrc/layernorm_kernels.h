@@ -1,6 +1,7 @@
 // Kernels of the layer norm, of the 8-bit form of activations, and of sums
 // over rows.
 #pragma once
+#include <hip/hip_runtime.h>
 #include "ffn_common.h"
 
 // ---- reductions --------------------------------------------------------------

@@ -1,6 +1,7 @@
 // Products of linear layers: choice of tile and of the split over k, launches.
+#include <hip/hip_runtime.h>
 #include "ffn_ops.h"
-#include <ATen/cuda/CUDAContext.h>
+#include <c10/hip/HIPStream.h>
 #include "linear_kernels.h"
 
 namespace ffn {
@@ -19,7 +20,7 @@ at::Tensor sum_partials(const at::Tensor& part, long long n, long long width,
                         at::ScalarType type);
 
 static hipStream_t stream_now() {
-    return at::cuda::getCurrentCUDAStream().stream();
+    return c10::hip::getCurrentHIPStream().stream();
 }
 
 struct Plan { int tile, splits; };
@@ -85,7 +86,7 @@ static void launch(const Operand& a, const Operand& b, int M, int N, int K,
     float* pp = parts > 1 ? part.data_ptr<float>() : nullptr;
     const dim3 grid((unsigned)(tm * tn), (unsigned)parts);
     auto k = gemm_kernel<T, BM, BN, WM, WN, AA, BA, EPI>;
-    k<<<grid, G::THREADS, G::LDS, s>>>(a, b, M, N, K, per * G::BK, pp,
+    hipLaunchKernelGGL(k, grid, G::THREADS, G::LDS, s, a, b, M, N, K, per * G::BK, pp,
                                        ld_part, e);
     FFN_OK();
     *blocks = tm;
@@ -93,7 +94,7 @@ static void launch(const Operand& a, const Operand& b, int M, int N, int K,
         const dim3 fgrid((unsigned)((M + FINISH_ROWS - 1) / FINISH_ROWS),
                          (unsigned)((N + 127) / 128));
         auto f = finish_kernel<T, EPI, float>;
-        f<<<fgrid, 256, 0, s>>>(pp, ld_part, parts, M, N, e);
+        hipLaunchKernelGGL(f, fgrid, 256, 0, s, pp, ld_part, parts, M, N, e);
         FFN_OK();
         *blocks = fgrid.x;
     }
@@ -228,7 +229,7 @@ Mat through_act(const Mat& dy, int act, const Kept& u, const at::Tensor& bias,
                     (unsigned)((p.dim + 127) / 128));
     FFN_TYPES(dy.t.scalar_type(),
         auto f = finish_kernel<T, EPI_GRAD, T>;
-        f<<<grid, 256, 0, stream_now()>>>((const T*)dy.t.data_ptr(), dy.ld, 1,
+        hipLaunchKernelGGL(f, grid, 256, 0, stream_now(), (const T*)dy.t.data_ptr(), dy.ld, 1,
                                           (int)p.rows, (int)p.dim, e));
     FFN_OK();
     if (bias.defined())

@@ -1,6 +1,7 @@
 // Kernels of linear layers: products with their epilogues, and the
 // joining of products that were split over k.
 #pragma once
+#include <hip/hip_runtime.h>
 #include "gemm.h"
 
 enum Epilogue { EPI_FORWARD = 0, EPI_GRAD = 1, EPI_PLAIN = 2 };
