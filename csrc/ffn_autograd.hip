@@ -110,11 +110,11 @@ struct NormFn : public torch::autograd::Function<NormFn> {
         const Mat m = as_rows(x);
         NormOut o = norm_forward(m, contiguous_or_none(gamma),
                                  contiguous_or_none(beta), eps, true, act8,
-                                 false);
+                                 false, false);
         ctx->save_for_backward({act8 ? Tensor() : x, gamma, beta, o.mean,
                                 o.rstd, o.x8.codes, o.x8.scales});
         ctx->saved_data["inputs"] = present({x, gamma, beta});
-        return o.y.view(x.sizes());
+        return o.y.t.view(x.sizes());
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -142,8 +142,8 @@ Tensor layer_norm(Tensor x, c10::optional<Tensor> weight,
     if (recording({x, gamma, beta}))
         return NormFn::apply(x, maybe(gamma), maybe(beta), eps, act8);
     return norm_forward(as_rows(x), contiguous_or_none(gamma),
-                        contiguous_or_none(beta), eps, false, false, false)
-        .y.view(x.sizes());
+                        contiguous_or_none(beta), eps, false, false, false,
+                        false).y.t.view(x.sizes());
 }
 
 // ---- linear layer ----------------------------------------------------------------
@@ -165,7 +165,7 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
                              wants_grad(bias);
         LinearOut o = linear_forward(m, as_rows(w), contiguous_or_none(bias),
                                      res.defined() ? &r : nullptr, (int)act,
-                                     through, act8, false);
+                                     through, act8, false, false);
         Packed x8;
         if (wants_grad(w) && act8) x8 = pack(m);
         ctx->save_for_backward({wants_grad(w) && !act8 ? x : Tensor(),
@@ -174,7 +174,7 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
         ctx->saved_data["inputs"] = present({x, w, bias, res});
         ctx->saved_data["act"] = act;
         ctx->saved_data["how"] = (int64_t)o.u.how;
-        return o.y.view(out_sizes(x, w.size(0)));
+        return o.y.t.view(out_sizes(x, w.size(0)));
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -194,8 +194,9 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
             Mat p = through_act(as_rows(dy), act, u, need_b ? s[6] : Tensor(),
                                 &db, act8);
             if (need_w)
-                dw = weight_grad(p, as_rows(
-                    act8 ? unpack(s[2], s[3], dy.scalar_type()) : s[0]));
+                dw = weight_grad(p, act8
+                    ? unpack(s[2], s[3], dy.scalar_type(), true)
+                    : as_rows(s[0]));
             p.lo = Tensor();
             if (need_x)
                 dx = input_grad(p, as_rows(s[1]), 0, Kept(), Tensor(), nullptr,
@@ -227,8 +228,8 @@ Tensor linear_act(Tensor x, Tensor weight, c10::optional<Tensor> bias,
     if (r.defined()) rm = as_rows(r);
     return linear_forward(as_rows(x), as_rows(weight), contiguous_or_none(b),
                           r.defined() ? &rm : nullptr, (int)act, false, false,
-                          false)
-        .y.view(out_sizes(x, weight.size(0)));
+                          false, false)
+        .y.t.view(out_sizes(x, weight.size(0)));
 }
 
 // ---- the block ---------------------------------------------------------------------
@@ -243,23 +244,22 @@ struct BlockFn : public torch::autograd::Function<BlockFn> {
         const Mat m = as_rows(x);
         NormOut n = norm_forward(m, contiguous_or_none(gamma),
                                  contiguous_or_none(beta), eps, true, act8,
-                                 act8);
-        LinearOut a = linear_forward(as_rows(n.y), as_rows(w1),
-                                     contiguous_or_none(b1), nullptr, (int)act,
-                                     true, act8, act8);
-        LinearOut o = linear_forward(as_rows(a.y), as_rows(w2),
-                                     contiguous_or_none(b2), &m, 0, false,
-                                     false, false);
+                                 act8, true);
+        LinearOut a = linear_forward(n.y, as_rows(w1), contiguous_or_none(b1),
+                                     nullptr, (int)act, true, act8, act8,
+                                     true);
+        LinearOut o = linear_forward(a.y, as_rows(w2), contiguous_or_none(b2),
+                                     &m, 0, false, false, false, false);
         const Tensor none;
         ctx->save_for_backward(
-            {act8 ? none : x, act8 ? none : n.y, act8 ? none : a.y, n.x8.codes,
+            {act8 ? none : x, act8 ? none : n.y.t, act8 ? none : a.y.t, n.x8.codes,
              n.x8.scales, n.y8.codes, n.y8.scales, a.y8.codes, a.y8.scales,
              a.u.data, a.u.scales, n.mean, n.rstd, gamma, beta, w1, b1, w2,
              b2});
         ctx->saved_data["inputs"] = present({x, gamma, beta, w1, b1, w2, b2});
         ctx->saved_data["act"] = act;
         ctx->saved_data["how"] = (int64_t)a.u.how;
-        return o.y.view(x.sizes());
+        return o.y.t.view(x.sizes());
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -272,8 +272,9 @@ struct BlockFn : public torch::autograd::Function<BlockFn> {
         const Tensor &w1 = s[15], &b1 = s[16], &w2 = s[17], &b2 = s[18];
         auto need = [&](int i) { return needs(ctx, i); };
         auto kept = [&](int plain, int packed) {
-            return as_rows(s[plain].defined()
-                ? s[plain] : unpack(s[packed], s[packed + 1], type));
+            return s[plain].defined()
+                ? as_rows(s[plain])
+                : unpack(s[packed], s[packed + 1], type, true);
         };
         Tensor dx, dw1, db1, dw2, db2;
         NormGrads g;
@@ -331,12 +332,12 @@ Tensor ffn_block(Tensor x, c10::optional<Tensor> norm_weight,
     const Mat m = as_rows(x);
     const NormOut n = norm_forward(m, contiguous_or_none(gamma),
                                    contiguous_or_none(beta), eps, false, false,
-                                   false);
-    const LinearOut a = linear_forward(as_rows(n.y), as_rows(w1),
-                                       contiguous_or_none(c1), nullptr,
-                                       (int)act, false, false, false);
-    return linear_forward(as_rows(a.y), as_rows(w2), contiguous_or_none(c2),
-                          &m, 0, false, false, false).y.view(x.sizes());
+                                   false, true);
+    const LinearOut a = linear_forward(n.y, as_rows(w1), contiguous_or_none(c1),
+                                       nullptr, (int)act, false, false, false,
+                                       true);
+    return linear_forward(a.y, as_rows(w2), contiguous_or_none(c2), &m, 0,
+                          false, false, false, false).y.t.view(x.sizes());
 }
 
 // ---- the 8-bit form ------------------------------------------------------------------
@@ -370,8 +371,8 @@ Tensor act8_unpack(Tensor codes, Tensor scales, int64_t type) {
                                                       : at::kHalf;
     const int64_t rows = codes.numel() / dim;
     return unpack(codes.contiguous().view({rows, dim}),
-                  scales.contiguous().view({rows, s.back()}), t)
-        .view(codes.sizes());
+                  scales.contiguous().view({rows, s.back()}), t, false)
+        .t.view(codes.sizes());
 }
 
 }  // namespace ffn

@@ -50,6 +50,44 @@ __device__ __forceinline__ void load8(const T* p, int left, float* v) {
     }
 }
 
+// 8 values from column c of a row of `dim`, as they lie in memory, for rows that
+// may end inside a chunk: nothing branches between the load and its use, so that
+// many are on their way at once.  Where the chunk ends past the row, its last 8
+// values come instead, and unpack8() moves them; `c` may lie past the row.
+template <typename T>
+__device__ __forceinline__ typename Chunk<T>::V fetch8(const T* row, int c,
+                                                       int dim) {
+    if (dim >= 8)
+        return *reinterpret_cast<const typename Chunk<T>::V*>(
+            row + (c < dim - 8 ? c : dim - 8));
+    typename Chunk<T>::V v;
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < dim ? row[i] : (T)0.0f;
+    return v;
+}
+
+// columns that are not there become 0.  `whole`: no lane's chunk ends past the
+// row (the same for all lanes).
+__device__ __forceinline__ void settle8(int c, int dim, bool whole, float* v) {
+    if (whole) return;
+    const int by = dim >= 8 && c > dim - 8 ? c - (dim - 8) : 0;
+    #pragma unroll
+    for (int b = 1; b < 8; b *= 2)
+        #pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = by & b ? (i + b < 8 ? v[i + b] : 0.0f) : v[i];
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + i < dim ? v[i] : 0.0f;
+}
+
+template <typename V>
+__device__ __forceinline__ void unpack8(V raw, int c, int dim, bool whole,
+                                        float* v) {
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)raw[i];
+    settle8(c, dim, whole, v);
+}
+
 template <typename T>
 __device__ __forceinline__ void store8(T* p, int left, const float* v) {
     if (left >= 8) {
@@ -120,11 +158,33 @@ __device__ __forceinline__ void store8_codes(signed char* p, int left,
     }
 }
 
-// max over 16 neighbouring lanes (one group of 128 values, 8 a lane)
+// lane values moved within the wave by the vector unit itself: a few cycles,
+// where a shuffle by way of LDS takes about a hundred
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float moved(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(
+        0, __float_as_int(v), CTRL, ROWS, 0xf, true));
+}
+
+// max over 16 neighbouring lanes (one group of 128 values, 8 a lane): each lane
+// takes in the one 8, 4, 2 and 1 lanes round
 __device__ __forceinline__ float max16(float a) {
-    #pragma unroll
-    for (int d = 1; d < 16; d <<= 1) a = fmaxf(a, __shfl_xor(a, d));
-    return a;
+    a = fmaxf(a, moved<0x128, 0xf>(a));
+    a = fmaxf(a, moved<0x124, 0xf>(a));
+    a = fmaxf(a, moved<0x122, 0xf>(a));
+    return fmaxf(a, moved<0x121, 0xf>(a));
+}
+
+// sum over the wave, the same in all lanes: over 16 lanes from the left, then
+// row 0 onto 1 and 2 onto 3, then the lower half onto the upper
+__device__ __forceinline__ float wave_sum(float v) {
+    v += moved<0x111, 0xf>(v);
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    v += moved<0x142, 0xa>(v);
+    v += moved<0x143, 0xc>(v);
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
 // ---- activations -----------------------------------------------------------

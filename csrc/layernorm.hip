@@ -58,37 +58,80 @@ Packed empty_packed(long long rows, long long dim, const at::Tensor& like) {
             at::empty({rows, groups_in(dim)}, like.options().dtype(at::kFloat))};
 }
 
+// 64-bit divisions take long: runs the statement with I as the type that counts
+// n pieces, and some blocks more
+#define FFN_COUNT(n, ...) do { \
+    if ((n) < (1LL << 30)) { typedef int I; __VA_ARGS__; } \
+    else { typedef long long I; __VA_ARGS__; } \
+} while (0)
+
 Packed pack(const Mat& x) {
     Packed p = empty_packed(x.rows, x.dim, x.t);
     const long long groups = x.rows * groups_in(x.dim);
     if (!groups) return p;
-    const int grid = (int)std::min<long long>((groups + 15) / 16, 256 * 16);
-    FFN_TYPES(x.t.scalar_type(),
-        auto k = act8_pack_kernel<T>;
-        hipLaunchKernelGGL(k, grid, 256, 0, stream_now(), (const T*)x.t.data_ptr(), x.ld, x.rows, (int)x.dim,
-            (signed char*)p.codes.data_ptr(),
-            p.scales.data_ptr<float>()));
+    const int grid = (int)std::min<long long>((groups + 63) / 64, 256 * 16);
+    FFN_TYPES(x.t.scalar_type(), FFN_COUNT(groups,
+        auto k = act8_pack_kernel<T, I>;
+        hipLaunchKernelGGL(k, grid, 256, 0, stream_now(),
+                           (const T*)x.t.data_ptr(), x.ld, (I)x.rows,
+                           (int)x.dim, (signed char*)p.codes.data_ptr(),
+                           p.scales.data_ptr<float>())));
     FFN_OK();
     return p;
 }
 
-at::Tensor unpack(const at::Tensor& codes, const at::Tensor& scales,
-                  at::ScalarType type) {
+Mat empty_rows(long long rows, long long dim, const at::Tensor& like,
+               at::ScalarType type) {
+    const long long line = 128 / c10::elementSize(type);
+    Mat m;
+    m.rows = rows;
+    m.dim = dim;
+    m.ld = dim < 4 * line ? dim : (dim + line - 1) / line * line;
+    m.t = at::empty({rows, m.ld}, like.options().dtype(type));
+    if (m.ld != dim) m.t = m.t.narrow(1, 0, dim);
+    return m;
+}
+
+Mat unpack(const at::Tensor& codes, const at::Tensor& scales,
+           at::ScalarType type, bool lines) {
     const long long rows = codes.size(0), dim = codes.size(1);
-    auto out = at::empty({rows, dim}, codes.options().dtype(type));
+    Mat out;
+    if (lines) {
+        out = empty_rows(rows, dim, codes, type);
+    } else {
+        out.t = at::empty({rows, dim}, codes.options().dtype(type));
+        out.rows = rows;
+        out.dim = out.ld = dim;
+    }
     const long long n = rows * ((dim + 7) / 8);
     if (!n) return out;
-    const int grid = (int)std::min<long long>((n + 255) / 256, 256 * 16);
-    FFN_TYPES(type,
-        auto k = act8_unpack_kernel<T>;
-        hipLaunchKernelGGL(k, grid, 256, 0, stream_now(), (const signed char*)codes.data_ptr(), scales.data_ptr<float>(),
-            rows, (int)dim, (T*)out.data_ptr()));
+    const int grid = (int)std::min<long long>((n + 1023) / 1024, 256 * 16);
+    FFN_TYPES(type, FFN_COUNT(n,
+        auto k = act8_unpack_kernel<T, I>;
+        hipLaunchKernelGGL(k, grid, 256, 0, stream_now(),
+                           (const signed char*)codes.data_ptr(),
+                           scales.data_ptr<float>(), (I)rows, (int)dim,
+                           (T*)out.t.data_ptr(), out.ld)));
     FFN_OK();
     return out;
 }
 
-// team of threads a row, chunks a thread: as few threads as hold the row in 4
-// chunks each (a wave: up to 2048 values; 256 threads: 8192; 1024: 32768)
+// team of threads a row, chunks of 8 a thread.  Forward: as few threads as hold
+// the row in 4 chunks each, so that a row of up to 2048 values needs no barrier.
+// Backward: as many threads as there are chunks, up to 1024, since a chunk takes
+// 32 registers there.  17920 x 1500 in bf16, x in 8 bits: 64 threads with 3
+// chunks 68 us (194 registers, two waves a unit), 256 with one BWD_US us.
+#define NORM_BACKWARD_SHAPES(dim, WIDE, GO) do { \
+    const long long chunks = ((dim) + 7) / 8; \
+    if (chunks <= 64) GO(64, 1); \
+    else if (chunks <= 128) GO(128, 1); \
+    else if (chunks <= 256) GO(256, 1); \
+    else if (chunks <= 512) GO(512, 1); \
+    else if (chunks <= 1024) GO(1024, 1); \
+    else if (chunks <= 2048) GO(1024, 2); \
+    else if (chunks <= 4096) GO(1024, 4); \
+    else WIDE; \
+} while (0)
 #define NORM_SHAPES(dim, WIDE, GO) do { \
     const long long chunks = ((dim) + 7) / 8; \
     if (chunks <= 64) GO(64, 1); \
@@ -104,9 +147,15 @@ at::Tensor unpack(const at::Tensor& codes, const at::Tensor& scales,
 
 NormOut norm_forward(const Mat& x, const at::Tensor& gamma,
                      const at::Tensor& beta, double eps, bool stats,
-                     bool keep_x8, bool keep_y8) {
+                     bool keep_x8, bool keep_y8, bool lines) {
     NormOut o;
-    o.y = at::empty({x.rows, x.dim}, x.t.options());
+    if (lines) {
+        o.y = empty_rows(x.rows, x.dim, x.t, x.t.scalar_type());
+    } else {
+        o.y.t = at::empty({x.rows, x.dim}, x.t.options());
+        o.y.rows = x.rows;
+        o.y.dim = o.y.ld = x.dim;
+    }
     const auto f32 = x.t.options().dtype(at::kFloat);
     if (stats) {
         o.mean = at::empty({x.rows}, f32);
@@ -122,7 +171,8 @@ NormOut norm_forward(const Mat& x, const at::Tensor& gamma,
     a.beta = beta.defined() ? beta.data_ptr() : nullptr;
     a.p32 = gamma.defined() ? gamma.scalar_type() == at::kFloat
           : beta.defined() && beta.scalar_type() == at::kFloat;
-    a.y = o.y.data_ptr();
+    a.y = o.y.t.data_ptr();
+    a.ld_y = o.y.ld;
     if (stats) {
         a.mean = o.mean.data_ptr<float>();
         a.rstd = o.rstd.data_ptr<float>();
@@ -213,12 +263,13 @@ NormGrads norm_backward(const Mat& x, const Packed& x8, const Mat& dy,
     #define GO(NT, R) do { \
         const int teams = NT == 64 ? 4 : 1, threads = NT == 64 ? 256 : NT; \
         blocks = std::min<long long>((rows + teams - 1) / teams, \
-                                     NT == 64 ? 768 : NT == 256 ? 512 : 256); \
+                                     NT <= 256 ? 1024 : NT == 512 ? 512 : 256); \
         if (params) { \
             part = at::empty({blocks, 2, dim}, f32); \
             a.part = part.data_ptr<float>(); \
         } \
-        auto k = norm_backward_kernel<T, NT, R>; \
+        auto k = a.x8 ? norm_backward_kernel<T, NT, R, true> \
+                      : norm_backward_kernel<T, NT, R, false>; \
         hipLaunchKernelGGL(k, (int)blocks, threads, 0, s, a); \
     } while (0)
     #define WIDE do { \
@@ -236,7 +287,7 @@ NormGrads norm_backward(const Mat& x, const Packed& x8, const Mat& dy,
             hipLaunchKernelGGL(k, grid, 256, 0, s, a, per); \
         } \
     } while (0)
-    FFN_TYPES(dy.t.scalar_type(), NORM_SHAPES(dim, WIDE, GO));
+    FFN_TYPES(dy.t.scalar_type(), NORM_BACKWARD_SHAPES(dim, WIDE, GO));
     #undef GO
     #undef WIDE
     FFN_OK();

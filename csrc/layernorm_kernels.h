@@ -5,12 +5,6 @@
 #include "ffn_common.h"
 
 // ---- reductions --------------------------------------------------------------
-__device__ __forceinline__ float wave_sum(float v) {
-    #pragma unroll
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-    return v;
-}
-
 // sums of two values over the NT threads of a team (a wave or a block).  slot:
 // 2 * 16 floats that no thread still reads; blocks alternate between two.
 template <int NT>
@@ -33,7 +27,8 @@ struct NormArgs {
     long long ld;
     const void* gamma;    // [dim] of T, or of float where p32; null: ones
     const void* beta;     // null: zeros
-    void* y;              // [rows, dim]
+    void* y;              // [rows, dim], rows ld_y apart
+    long long ld_y;
     float* mean;          // [rows], with rstd; null: not kept
     float* rstd;
     signed char* x8;      // 8-bit form of x, or null
@@ -106,10 +101,14 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_forward_kernel(
          row += gridDim.x * TEAMS) {
         const T* x = (const T*)p.x + row * p.ld;
         float v[R][8], s = 0.0f, q = 0.0f, none = 0.0f;
+        typename Chunk<T>::V raw[R];
+        #pragma unroll
+        for (int i = 0; i < R; ++i)
+            raw[i] = fetch8(x, (i * NT + t) * 8, p.dim);
         #pragma unroll
         for (int i = 0; i < R; ++i) {
-            const int c = (i * NT + t) * 8;
-            load8(x + c, p.dim - c, v[i]);
+            unpack8(raw[i], (i * NT + t) * 8, p.dim,
+                    (i + 1) * NT * 8 <= p.dim, v[i]);
             #pragma unroll
             for (int j = 0; j < 8; ++j) s += v[i][j];
         }
@@ -136,7 +135,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_forward_kernel(
             for (int j = 0; j < 8; ++j)
                 v[i][j] = (v[i][j] - mean) * rstd * g[i][j] + b[i][j];
             if (left > 0)
-                store8((T*)p.y + (long long)row * p.dim + c, left, v[i]);
+                store8((T*)p.y + row * p.ld_y + c, left, v[i]);
             if (p.y8) {
                 #pragma unroll
                 for (int j = 0; j < 8; ++j)
@@ -164,6 +163,49 @@ struct NormGradArgs {
     int rows, dim, p32;
 };
 
+// 8 columns of the kept x as they lie in memory: values, or codes with their
+// group's scale
+template <typename T, bool X8> struct KeptRaw {
+    typename Chunk<T>::V raw;
+    __device__ __forceinline__ void fetch(const NormGradArgs& p, int row,
+                                          int c) {
+        raw = fetch8((const T*)p.x + row * p.ld, c, p.dim);
+    }
+    __device__ __forceinline__ void unpack(int c, int dim, bool whole,
+                                           float* v) const {
+        unpack8(raw, c, dim, whole, v);
+    }
+    __device__ __forceinline__ void renew() { asm volatile("" : "+v"(raw)); }
+};
+template <typename T> struct KeptRaw<T, true> {
+    u32x2 raw;
+    float scale;
+    __device__ __forceinline__ void fetch(const NormGradArgs& p, int row_,
+                                          int c) {
+        const long long row = row_;
+        const signed char* q = p.x8 + row * p.dim;
+        i8x8 r;
+        if (p.dim >= 8) {
+            r = *reinterpret_cast<const i8x8*>(
+                q + (c < p.dim - 8 ? c : p.dim - 8));
+        } else {
+            #pragma unroll
+            for (int i = 0; i < 8; ++i)
+                r[i] = i < p.dim ? q[i] : (signed char)0;
+        }
+        raw = __builtin_bit_cast(u32x2, r);
+        const int g = c < p.dim ? c / ACT8_GROUP : groups_of(p.dim) - 1;
+        scale = p.x8_scale[row * groups_of(p.dim) + g];
+    }
+    __device__ __forceinline__ void unpack(int c, int dim, bool whole,
+                                           float* v) const {
+        unpack8(__builtin_bit_cast(i8x8, raw), c, dim, whole, v);
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= scale;
+    }
+    __device__ __forceinline__ void renew() { asm volatile("" : "+v"(raw)); }
+};
+
 template <typename T>
 __device__ __forceinline__ void load_kept(const NormGradArgs& p, long long row,
                                           int c, int left, float* v) {
@@ -179,10 +221,10 @@ __device__ __forceinline__ void load_kept(const NormGradArgs& p, long long row,
 // each thread sums dy xh and dy for its own columns over the rows that it
 // sees, the teams of a block add theirs in turn, and column_sum_kernel adds
 // the blocks': no atomics, the same result each time.
-template <typename T, int NT, int R>
-__global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_backward_kernel(
+template <typename T, int NT, int R, bool X8>
+__global__ __launch_bounds__(NT < 128 ? 256 : NT) void norm_backward_kernel(
         NormGradArgs p) {
-    constexpr int TEAMS = NT < 256 ? 256 / NT : 1;
+    constexpr int TEAMS = NT < 128 ? 256 / NT : 1;
     __shared__ float slots[2][32];
     __shared__ float all[TEAMS > 1 ? 2 * NT * R * 8 : 1];
     const int t = threadIdx.x % NT, team = threadIdx.x / NT;
@@ -199,24 +241,35 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_backward_kernel(
     for (int row = blockIdx.x * TEAMS + team; row < p.rows;
          row += gridDim.x * TEAMS, turn ^= 1) {
         const float mean = p.mean[row], rstd = p.rstd[row];
-        float h[R][8], d[R][8], s1 = 0.0f, s2 = 0.0f;
+        float s1 = 0.0f, s2 = 0.0f;
+        KeptRaw<T, X8> rh[R];
+        typename Chunk<T>::V rd[R];
         #pragma unroll
         for (int i = 0; i < R; ++i) {
-            const int c = (i * NT + t) * 8, left = p.dim - c;
-            load_kept<T>(p, row, c, left, h[i]);
-            load8((const T*)p.dy + row * p.ld_dy + c, left, d[i]);
+            const int c = (i * NT + t) * 8;
+            rh[i].fetch(p, row, c);
+            rd[i] = fetch8((const T*)p.dy + row * p.ld_dy, c, p.dim);
         }
+        // xh and dy of a chunk; columns that are not there have dy = 0
+        auto values = [&](int i, float* h, float* d) {
+            const int c = (i * NT + t) * 8;
+            const bool whole = (i + 1) * NT * 8 <= p.dim;
+            rh[i].unpack(c, p.dim, whole, h);
+            unpack8(rd[i], c, p.dim, whole, d);
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) h[j] = (h[j] - mean) * rstd;
+        };
         #pragma unroll
         for (int i = 0; i < R; ++i) {
+            float h[8], d[8];
+            values(i, h, d);
             #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                // columns that are not there have dy = 0
-                h[i][j] = (h[i][j] - mean) * rstd;
-                sg[i][j] += d[i][j] * h[i][j];
-                sb[i][j] += d[i][j];
-                d[i][j] *= g[i][j];
-                s1 += d[i][j];
-                s2 += d[i][j] * h[i][j];
+                sg[i][j] += d[j] * h[j];
+                sb[i][j] += d[j];
+                d[j] *= g[i][j];
+                s1 += d[j];
+                s2 += d[j] * h[j];
             }
         }
         if (!p.dx) continue;
@@ -225,16 +278,23 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_backward_kernel(
         s2 *= inv;
         #pragma unroll
         for (int i = 0; i < R; ++i) {
+            // unpacked anew: kept as 32 bits, the row would take the registers
+            // of a second wave
+            asm volatile("" : "+v"(rd[i]));
+            rh[i].renew();
             const int c = (i * NT + t) * 8, left = p.dim - c;
-            if (left <= 0) continue;
-            float a[8];
-            if (p.add) load8((const T*)p.add + row * p.ld_add + c, left, a);
+            float h[8], d[8], a[8];
+            values(i, h, d);
+            if (p.add)
+                unpack8(fetch8((const T*)p.add + row * p.ld_add, c, p.dim), c,
+                        p.dim, (i + 1) * NT * 8 <= p.dim, a);
             #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float v = rstd * (d[i][j] - s1 - h[i][j] * s2);
-                d[i][j] = p.add ? v + a[j] : v;
+                const float v = rstd * (d[j] * g[i][j] - s1 - h[j] * s2);
+                d[j] = p.add ? v + a[j] : v;
             }
-            store8((T*)p.dx + (long long)row * p.dim + c, left, d[i]);
+            if (left > 0)
+                store8((T*)p.dx + (long long)row * p.dim + c, left, d);
         }
     }
     if (!p.part) return;
@@ -305,7 +365,7 @@ __global__ __launch_bounds__(1024) void norm_forward_wide_kernel(NormArgs p) {
         load_param<T>(p.beta, p.p32, c, left, 0.0f, b);
         #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = (v[j] - mean) * rstd * g[j] + b[j];
-        if (left > 0) store8((T*)p.y + (long long)row * p.dim + c, left, v);
+        if (left > 0) store8((T*)p.y + row * p.ld_y + c, left, v);
         if (p.y8) {
             #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -363,10 +423,12 @@ __global__ __launch_bounds__(256) void row_sum_kernel(NormGradArgs p,
     const int last = p.rows - first < per ? p.rows : first + per;
     float sg[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sb[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (left > 0) {
-        #pragma unroll 4
+        const bool whole = (blockIdx.x + 1) * 256 <= p.dim;
+        #pragma unroll 8
         for (int row = first + r0; row < last; row += 8) {
             float d[8], h[8];
-            load8((const T*)p.dy + row * p.ld_dy + c, left, d);
+            unpack8(fetch8((const T*)p.dy + row * p.ld_dy, c, p.dim), c, p.dim,
+                    whole, d);
             if (NORM) {
                 load_kept<T>(p, row, c, left, h);
                 #pragma unroll
@@ -417,38 +479,76 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(
 }
 
 // ---- the 8-bit form by itself ------------------------------------------------------
-template <typename T>
+// A group of 128 values for each 16 lanes, GROUPS of them at a time; I is the
+// type that counts them.
+template <typename T, typename I>
 __global__ __launch_bounds__(256) void act8_pack_kernel(
-        const T* x, long long ld, long long rows, int dim, signed char* codes,
+        const T* x, long long ld, I rows, int dim, signed char* codes,
         float* scales) {
-    const int ng = groups_of(dim);
-    const long long groups = rows * ng, step = (long long)gridDim.x * 16;
+    constexpr int GROUPS = 4;
+    const I ng = groups_of(dim), groups = rows * ng;
+    const int t = threadIdx.x >> 4, o = (threadIdx.x & 15) * 8;
     // all lanes of a wave go round as often, for max16
-    for (long long g0 = (long long)blockIdx.x * 16; g0 < groups; g0 += step) {
-        const long long g = g0 + (threadIdx.x >> 4);
-        const bool on = g < groups;
-        const long long row = on ? g / ng : 0;
-        const int c = (int)(g - row * ng) * ACT8_GROUP + (threadIdx.x & 15) * 8;
-        const int left = on ? dim - c : 0;
-        float v[8];
-        load8(x + row * ld + c, left, v);
-        keep8(codes, scales, row, c, left, dim, v);
+    for (I g0 = (I)blockIdx.x * 16 * GROUPS; g0 < groups;
+         g0 += (I)gridDim.x * 16 * GROUPS) {
+        typename Chunk<T>::V raw[GROUPS];
+        I row[GROUPS];
+        int c[GROUPS];
+        #pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+            const I at = g0 + i * 16 + t, g = at < groups ? at : groups - 1;
+            row[i] = g / ng;
+            c[i] = (int)(g - row[i] * ng) * ACT8_GROUP + o;
+            raw[i] = fetch8(x + (long long)row[i] * ld, c[i], dim);
+            if (at >= groups) c[i] = dim;
+        }
+        #pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+            float v[8];
+            unpack8(raw[i], c[i], dim, dim % ACT8_GROUP == 0, v);
+            keep8(codes, scales, row[i], c[i], dim - c[i], dim, v);
+        }
     }
 }
 
-template <typename O>
+// Values of 8 bits to 16 or 32, rows ld apart.
+template <typename O, typename I>
 __global__ __launch_bounds__(256) void act8_unpack_kernel(
-        const signed char* codes, const float* scales, long long rows, int dim,
-        O* out) {
-    const int nc = (dim + 7) / 8;
-    const long long n = rows * nc, step = (long long)gridDim.x * 256;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n;
-         i += step) {
-        const long long row = i / nc;
-        const int c = (int)(i - row * nc) * 8;
-        float v[8];
-        load8_codes(codes + row * dim + c, dim - c,
-                    scales[row * groups_of(dim) + c / ACT8_GROUP], v);
-        store8(out + row * dim + c, dim - c, v);
+        const signed char* codes, const float* scales, I rows, int dim, O* out,
+        long long ld) {
+    constexpr int CHUNKS = 4;
+    const I nc = (dim + 7) / 8, n = rows * nc;
+    const int ng = groups_of(dim);
+    for (I i0 = (I)blockIdx.x * 256 * CHUNKS + threadIdx.x; i0 < n;
+         i0 += (I)gridDim.x * 256 * CHUNKS) {
+        i8x8 raw[CHUNKS];
+        float scale[CHUNKS];
+        I row[CHUNKS];
+        int c[CHUNKS];
+        #pragma unroll
+        for (int k = 0; k < CHUNKS; ++k) {
+            const I at = i0 + k * 256, i = at < n ? at : n - 1;
+            row[k] = i / nc;
+            c[k] = (int)(i - row[k] * nc) * 8;
+            const signed char* p = codes + (long long)row[k] * dim;
+            if (dim >= 8) {
+                raw[k] = *reinterpret_cast<const i8x8*>(
+                    p + (c[k] < dim - 8 ? c[k] : dim - 8));
+            } else {
+                #pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    raw[k][j] = j < dim ? p[j] : (signed char)0;
+            }
+            scale[k] = scales[(long long)row[k] * ng + c[k] / ACT8_GROUP];
+        }
+        #pragma unroll
+        for (int k = 0; k < CHUNKS; ++k) {
+            if (i0 + k * 256 >= n) break;
+            float v[8];
+            unpack8(raw[k], c[k], dim, dim % 8 == 0, v);
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] *= scale[k];
+            store8(out + (long long)row[k] * ld + c[k], dim - c[k], v);
+        }
     }
 }

@@ -23,19 +23,31 @@ static hipStream_t stream_now() {
     return c10::hip::getCurrentHIPStream().stream();
 }
 
+// up to this many rows go to thin_kernel where it has a form for the operands
+#define THIN_ROWS 64
+
 struct Plan { int tile, splits; };
 
-// Estimated time in us of the product with each tile and split, the least one
-// wins.  A tile's step over 128 bytes of k takes `step` us while `at_once`
-// blocks share a compute unit; `over` is what a block spends outside its loop.
+// Estimated us of the product with each tile and number of parts of k; the
+// least one wins.  A tile's step over 128 bytes of k takes `step` us, `more`
+// longer for each further block (up to `at_once`) that shares its compute unit,
+// and a block spends `over` us outside its loop; parts cost `join` us and their
+// way to memory and back at `rate` bytes a us.  The numbers fit 74 products of
+// 1 to 17920 rows, each timed with all tiles and up to 16 parts: the choice is
+// 1.5 % slower than the best one in the mean, and 19 % at worst.
 static Plan plan_product(long long M, long long N, long long K, int size,
                          bool quantises) {
-    struct Shape { int tile, at_once; float step, over; };
-    static const Shape half[] = {{256, 1, 1.75f, 6.0f}, {128, 2, 1.0f, 4.0f},
-                                 {64, 5, 0.8f, 3.0f}};
-    static const Shape full[] = {{128, 2, 4.0f, 5.0f}, {64, 5, 2.6f, 3.0f}};
+    struct Shape { int tile, at_once; float over, step, more; };
+    static const Shape half[] = {{256, 1, 10.3f, 1.16f, 0.0f},
+                                 {128, 2, 4.5f, 0.65f, 0.24f},
+                                 {64, 5, 3.05f, 0.284f, 0.177f}};
+    static const Shape full[] = {{128, 2, 5.6f, 1.8f, 0.58f},
+                                 {64, 5, 3.05f, 0.49f, 0.33f}};
     const Shape* shapes = size == 2 ? half : full;
     const int n = size == 2 ? 3 : 2;
+    const float join = size == 2 ? 5.3f : 3.2f;
+    const float rate = size == 2 ? 5.44e6f : 3.3e6f;
+    const long long units = 256;
     const long long steps = (K * size + 127) / 128;
     Plan best{shapes[0].tile, 1};
     float least = 1e30f;
@@ -44,25 +56,28 @@ static Plan plan_product(long long M, long long N, long long K, int size,
         if (quantises && s.tile < ACT8_GROUP) continue;
         const long long tiles = ((M + s.tile - 1) / s.tile) *
                                 ((N + s.tile - 1) / s.tile);
-        for (int splits = 1; splits <= 16 && splits <= steps; ++splits) {
-            const long long per = (steps + splits - 1) / splits;
-            const long long parts = (steps + per - 1) / per;
-            if (parts != splits) continue;
-            const long long all = tiles * splits;
-            const long long slots = 256LL * s.at_once;
-            const long long rounds = (all + slots - 1) / slots;
-            // a last round that is not full runs with fewer blocks a unit
-            float t = rounds * (per * s.step + s.over);
-            if (all < slots) {
-                const float share = (float)((all + 255) / 256) / s.at_once;
-                t = per * s.step * (0.5f + 0.5f * share) + s.over;
-            }
-            if (splits > 1)
-                t += 4.0f + (float)M * N * 4.0f * (2 * splits) / 4.0e6f;
-            if (t < least) { least = t; best = {s.tile, splits}; }
+        for (int parts = 1; parts <= 16 && parts <= steps; ++parts) {
+            const long long per = (steps + parts - 1) / parts;
+            if ((steps + per - 1) / per != parts) continue;
+            const long long all = tiles * parts, slots = units * s.at_once;
+            const long long rest = all % slots;
+            float t = all / slots *
+                (per * (s.step + s.more * (s.at_once - 1)) + s.over);
+            if (rest)
+                t += per * (s.step + s.more * ((rest - 1) / units)) + s.over;
+            if (parts > 1) t += join + 8.0f * M * N * parts / rate;
+            if (t < least) { least = t; best = {s.tile, parts}; }
         }
     }
     return best;
+}
+
+// rows a block of finish_kernel: as many as leave it 512 blocks, up to 64
+static int finish_rows(long long M, long long N) {
+    int rows = 64;
+    while (rows > 16 && (M + rows - 1) / rows * ((N + 127) / 128) < 512)
+        rows /= 2;
+    return rows;
 }
 
 template <typename T, int BM, int BN, int WM, int WN, bool AA, bool BA,
@@ -91,10 +106,12 @@ static void launch(const Operand& a, const Operand& b, int M, int N, int K,
     FFN_OK();
     *blocks = tm;
     if (parts > 1) {
-        const dim3 fgrid((unsigned)((M + FINISH_ROWS - 1) / FINISH_ROWS),
+        const int rows = finish_rows(M, N);
+        const dim3 fgrid((unsigned)((M + rows - 1) / rows),
                          (unsigned)((N + 127) / 128));
         auto f = finish_kernel<T, EPI, float>;
-        hipLaunchKernelGGL(f, fgrid, 256, 0, s, pp, ld_part, parts, M, N, e);
+        hipLaunchKernelGGL(f, fgrid, 256, 0, s, pp, ld_part, parts, rows, M, N,
+                           e);
         FFN_OK();
         *blocks = fgrid.x;
     }
@@ -105,9 +122,27 @@ template <bool AA, bool BA, int EPI>
 static void product(at::ScalarType type, const Operand& a, const Operand& b,
                     long long M, long long N, long long K, EpiArgs e,
                     const at::Tensor& like, long long* blocks) {
-    const bool quantises = e.out8 || e.keep == KEEP_8BIT;
-    const Plan p = plan_product(M, N, a.lo ? 2 * K : K, type == at::kFloat ? 4 : 2,
-                                EPI == EPI_FORWARD && quantises);
+    const bool quantises = EPI == EPI_FORWARD &&
+                           (e.out8 || e.keep == KEEP_8BIT);
+    if constexpr (AA) {
+        if (M <= THIN_ROWS && !quantises && !a.lo &&
+            (BA || type == at::kFloat)) {
+            const dim3 grid((unsigned)((N + 31) / 32),
+                            (unsigned)((M + 31) / 32));
+            FFN_TYPES(type,
+                if constexpr (BA || sizeof(T) == 4) {
+                    auto k = thin_kernel<T, BA, EPI>;
+                    hipLaunchKernelGGL(k, grid, THIN_WAVES * 64, 0,
+                                       stream_now(), a, b, (int)M, (int)N,
+                                       (int)K, e);
+                });
+            FFN_OK();
+            *blocks = grid.y;
+            return;
+        }
+    }
+    const Plan p = plan_product(M, N, a.lo ? 2 * K : K,
+                                type == at::kFloat ? 4 : 2, quantises);
     FFN_TYPES(type,
         if (p.tile == 256) {
             if constexpr (sizeof(T) == 2)
@@ -153,16 +188,22 @@ static void set_kept(EpiArgs& e, const Kept& u) {
 
 LinearOut linear_forward(const Mat& x, const Mat& w, const at::Tensor& bias,
                          const Mat* res, int act, bool keep, bool act8,
-                         bool keep_y8) {
+                         bool keep_y8, bool lines) {
     LinearOut o;
     const long long M = x.rows, N = w.rows;
-    o.y = at::empty({M, N}, x.t.options());
+    if (lines) {
+        o.y = empty_rows(M, N, x.t, x.t.scalar_type());
+    } else {
+        o.y.t = at::empty({M, N}, x.t.options());
+        o.y.rows = M;
+        o.y.dim = o.y.ld = N;
+    }
     if (keep) o.u = empty_kept(act, act8, M, N, x.t);
     if (keep_y8) o.y8 = empty_packed(M, N, x.t);
     if (!M) return o;
     EpiArgs e{};
-    e.out = o.y.data_ptr();
-    e.ld_out = N;
+    e.out = o.y.t.data_ptr();
+    e.ld_out = o.y.ld;
     if (bias.defined()) {
         e.bias = bias.data_ptr();
         e.bias_f32 = bias.scalar_type() == at::kFloat;
@@ -186,20 +227,18 @@ LinearOut linear_forward(const Mat& x, const Mat& w, const at::Tensor& bias,
 // rows of partial sums that any tile may write
 static at::Tensor empty_colsum(long long rows, long long dim,
                                const at::Tensor& like) {
-    return at::empty({(rows + FINISH_ROWS - 1) / FINISH_ROWS, dim},
+    const int least = rows <= THIN_ROWS ? 16 : finish_rows(rows, dim);
+    return at::empty({(rows + least - 1) / least, dim},
                      like.options().dtype(at::kFloat));
 }
 
 static Mat empty_grad(long long rows, long long dim, const at::Tensor& like,
                       bool split, const Kept& u) {
-    Mat p;
-    p.t = at::empty({rows, dim}, like.options());
+    Mat p = empty_rows(rows, dim, like, like.scalar_type());
     // through relu a value passes whole; fp32 rounds as the sums themselves do
     if (split && (u.how == KEEP_FULL || u.how == KEEP_8BIT) &&
         like.scalar_type() != at::kFloat)
-        p.lo = at::empty({rows, dim}, like.options());
-    p.rows = rows;
-    p.dim = p.ld = dim;
+        p.lo = empty_rows(rows, dim, like, like.scalar_type()).t;
     return p;
 }
 
@@ -225,11 +264,12 @@ Mat through_act(const Mat& dy, int act, const Kept& u, const at::Tensor& bias,
         part = empty_colsum(p.rows, p.dim, p.t);
         e.colsum = part.data_ptr<float>();
     }
-    const dim3 grid((unsigned)((p.rows + FINISH_ROWS - 1) / FINISH_ROWS),
+    const int rows = finish_rows(p.rows, p.dim);
+    const dim3 grid((unsigned)((p.rows + rows - 1) / rows),
                     (unsigned)((p.dim + 127) / 128));
     FFN_TYPES(dy.t.scalar_type(),
         auto f = finish_kernel<T, EPI_GRAD, T>;
-        hipLaunchKernelGGL(f, grid, 256, 0, stream_now(), (const T*)dy.t.data_ptr(), dy.ld, 1,
+        hipLaunchKernelGGL(f, grid, 256, 0, stream_now(), (const T*)dy.t.data_ptr(), dy.ld, 1, rows,
                                           (int)p.rows, (int)p.dim, e));
     FFN_OK();
     if (bias.defined())
@@ -240,7 +280,14 @@ Mat through_act(const Mat& dy, int act, const Kept& u, const at::Tensor& bias,
 Mat input_grad(const Mat& p, const Mat& w, int act, const Kept& u,
                const at::Tensor& bias, at::Tensor* dbias, bool split) {
     const long long M = p.rows, N = w.dim;
-    Mat out = empty_grad(M, N, p.t, split, u);
+    Mat out;
+    if (act != ACT_NONE) {      // goes on into products
+        out = empty_grad(M, N, p.t, split, u);
+    } else {
+        out.t = at::empty({M, N}, p.t.options());
+        out.rows = M;
+        out.dim = out.ld = N;
+    }
     if (!M) {
         if (bias.defined()) *dbias = at::zeros_like(bias);
         return out;
@@ -248,7 +295,7 @@ Mat input_grad(const Mat& p, const Mat& w, int act, const Kept& u,
     EpiArgs e{};
     e.out = out.t.data_ptr();
     e.out_lo = out.lo.defined() ? out.lo.data_ptr() : nullptr;
-    e.ld_out = N;
+    e.ld_out = out.ld;
     e.act = act;
     set_kept(e, u);
     at::Tensor part;

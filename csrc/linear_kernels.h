@@ -146,19 +146,12 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(
     const int k0 = blockIdx.y * kper;
     const int k1 = K - k0 < kper ? K : k0 + kper;
 
-    f32x16 acc[G::TM][G::TN];
-    #pragma unroll
-    for (int i = 0; i < G::TM; ++i)
-        #pragma unroll
-        for (int j = 0; j < G::TN; ++j)
-            #pragma unroll
-            for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
-    for (;;) {
-        G::loop(lds, a, b, m0, n0, M, N, K, k0, k1, acc);
-        if (!a.lo) break;
-        a.p = a.lo;
-        a.lo = nullptr;
-        stage_wait();
+    G g(lds, a, b, M, N, K, m0, n0);
+    g.run(k0, k1);
+    if (a.lo) {
+        g.a.p = a.lo;
+        stage_wait<0>();
+        g.run(k0, k1);
     }
 
     constexpr int CH = BN / 8;             // chunks of 8 columns
@@ -169,7 +162,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(
     #pragma unroll
     for (int i = 0; i < G::TM; ++i) {
         __syncthreads();
-        G::stage_out(lds, i, acc[i]);
+        g.stage_out(lds, i);
         __syncthreads();
         for (int r = r0; r < WM * 32; r += RS) {
             const float* s = reinterpret_cast<const float*>(lds) +
@@ -202,23 +195,108 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(
     }
 }
 
-// Joins `splits` partial products, 64 rows x 128 columns a block, in the order
-// of k, and finishes them as the product's own epilogue would.  With one
-// "product" of type S it takes a gradient back through an activation.
-#define FINISH_ROWS 64
+// Few rows: 32 x 32 results a block, k shared out among its 8 waves.  The
+// fragments come straight from memory, 16 bytes a lane along k: there is nothing
+// to share, and no barrier before the end.  What bounds it is the weight's way
+// from memory.  BA false (32 bits only): a lane's 4 values of B lie across k.
+#define THIN_WAVES 8
+template <typename T, bool BA, int EPI>
+__global__ __launch_bounds__(THIN_WAVES * 64) void thin_kernel(
+        Operand a, Operand b, int M, int N, int K, EpiArgs e) {
+    static_assert(BA || sizeof(T) == 4, "across k needs 32 bits");
+    constexpr int E = 16 / sizeof(T), U = 2 * E, LD = 36;
+    typedef T V __attribute__((ext_vector_type(E), aligned(sizeof(T))));
+    __shared__ float part[THIN_WAVES][32][LD];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int row = lane & 31, off = E * (lane >> 5);
+    const int m0 = blockIdx.y * 32, n0 = blockIdx.x * 32;
+    // rows that are not there: the last one's values, for results not written
+    const long long ma = m0 + row < M ? m0 + row : M - 1;
+    const long long nb = n0 + row < N ? n0 + row : N - 1;
+    const T* pa = (const T*)a.p + ma * a.ld + off;
+    const T* pb = (const T*)b.p + (BA ? nb * b.ld + off : off * b.ld + nb);
+    const int steps = (K + U - 1) / U;
+    const int per = (steps + THIN_WAVES - 1) / THIN_WAVES;
+    const int s0 = wave * per, s1 = s0 + per < steps ? s0 + per : steps;
+    const int whole = K / U < s1 ? K / U : s1;
+    f32x16 acc;
+    #pragma unroll
+    for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
+    auto step = [&](int s, bool all) {
+        typename Mfma<T>::V x, y;
+        const int k = s * U;
+        if (all) {
+            x = *reinterpret_cast<const V*>(pa + k);
+        } else {
+            #pragma unroll
+            for (int i = 0; i < E; ++i)
+                x[i] = k + off + i < K ? pa[k + i] : (T)0.0f;
+        }
+        if (BA && all) {
+            y = *reinterpret_cast<const V*>(pb + k);
+        } else {
+            #pragma unroll
+            for (int i = 0; i < E; ++i)
+                y[i] = all || k + off + i < K
+                    ? pb[BA ? k + i : (long long)(k + i) * b.ld] : (T)0.0f;
+        }
+        acc = Mfma<T>::go(y, x, acc);
+    };
+    #pragma unroll 6
+    for (int s = s0; s < whole; ++s) step(s, true);
+    if (s0 < s1 && whole < s1) step(whole, false);
+    #pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        f32x4 v;
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = acc[4 * g + i];
+        *reinterpret_cast<f32x4*>(&part[wave][row][8 * g + 4 * (lane >> 5)]) = v;
+    }
+    __syncthreads();
+    const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 8;
+    float sums[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (threadIdx.x < 128) {
+        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        #pragma unroll
+        for (int w = 0; w < THIN_WAVES; ++w)
+            #pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += part[w][r][c + i];
+        finish8<T, EPI>(v, m0 + r, n0 + c, m0 + r < M ? N - n0 - c : 0, N, e,
+                        sums);
+    }
+    if (EPI == EPI_GRAD && e.colsum) {
+        __syncthreads();
+        if (threadIdx.x < 128) {
+            #pragma unroll
+            for (int i = 0; i < 8; ++i) part[0][r][c + i] = sums[i];
+        }
+        __syncthreads();
+        if (threadIdx.x < 32 && n0 + threadIdx.x < N) {
+            float t = 0.0f;
+            for (int i = 0; i < 32; ++i) t += part[0][i][threadIdx.x];
+            e.colsum[(long long)blockIdx.y * N + n0 + threadIdx.x] = t;
+        }
+    }
+}
+
+// Joins `splits` partial products, `rows` (a multiple of 16) x 128 columns a
+// block, in the order of k, and finishes them as the product's own epilogue
+// would.  With one "product" of type S it takes a gradient back through an
+// activation.
 template <typename T, int EPI, typename S>
 __global__ __launch_bounds__(256) void finish_kernel(
-        const S* part, long long ld_part, int splits, int M, int N,
+        const S* part, long long ld_part, int splits, int rows, int M, int N,
         EpiArgs e) {
     __shared__ float all[16 * 128];
     const int c = threadIdx.x & 15, r0 = threadIdx.x >> 4;
     const int n = blockIdx.y * 128 + 8 * c, left = N - n;
     float sums[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (int r = r0; r < FINISH_ROWS; r += 16) {
-        const long long m = (long long)blockIdx.x * FINISH_ROWS + r;
+    for (int r = r0; r < rows; r += 16) {
+        const long long m = (long long)blockIdx.x * rows + r;
         const int here = m < M ? left : 0;
         float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         if (here > 0) {
+            #pragma unroll 4
             for (int s = 0; s < splits; ++s) {
                 float w[8];
                 load8(part + ((long long)s * M + m) * ld_part + n, here, w);
