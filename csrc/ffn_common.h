@@ -188,49 +188,62 @@ __device__ __forceinline__ float wave_sum(float v) {
 }
 
 // ---- activations -----------------------------------------------------------
-// Phi(u), the normal distribution's integral, and phi(u) = exp(-u^2/2) /
-// sqrt(2 pi).  FAST: Abramowitz & Stegun 26.2.17 in the form of 7.1.26, one
-// exp and one reciprocal, |error| < 1.5e-7 absolute: under 2^-22, while the
-// 16-bit types it serves round to 2^-12 at best.  Otherwise erff.
+// q = Phi(-|u|), the normal distribution's tail, and e = exp(-u^2 / 2).  FAST:
+// Abramowitz & Stegun 7.1.26, erf(z) = 1 - t P(t) exp(-z^2) with t = 1 / (1 + p z)
+// and z = |u| / sqrt(2), |error| < 1.5e-7: under 2^-22, while the 16-bit types
+// that it serves round to 2^-12 at best.  One exp and one reciprocal; the
+// epilogues that use it are bound by the vector unit.  Otherwise erfcf.
 template <bool FAST>
-__device__ __forceinline__ void normal_cdf_pdf(float u, float* cdf,
-                                               float* pdf) {
-    const float e = FAST ? __expf(-0.5f * u * u) : expf(-0.5f * u * u);
-    *pdf = e * 0.3989422804014327f;
+__device__ __forceinline__ float normal_tail(float u, float* e) {
+    const float z = fabsf(u);
     if (FAST) {
-        const float z = fabsf(u) * 0.7071067811865476f;
-        const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * z);
-        const float q = t * (0.254829592f + t * (-0.284496736f +
-                        t * (1.421413741f + t * (-1.453152027f +
-                        t * 1.061405429f)))) * e * 0.5f;
-        *cdf = u < 0.0f ? q : 1.0f - q;
-    } else {
-        *cdf = 0.5f * (1.0f + erff(u * 0.7071067811865476f));
+        // exp2(-u^2 / 2 * log2(e))
+        *e = __builtin_amdgcn_exp2f(u * (u * -0.72134752044f));
+        // p / sqrt(2); the coefficients are halved
+        const float t = __builtin_amdgcn_rcpf(
+            __builtin_fmaf(z, 0.23164189f, 1.0f));
+        float q = __builtin_fmaf(t, 0.5307027145f, -0.7265760135f);
+        q = __builtin_fmaf(t, q, 0.7107068705f);
+        q = __builtin_fmaf(t, q, -0.142248368f);
+        q = __builtin_fmaf(t, q, 0.127414796f);
+        return q * t * *e;
     }
+    *e = expf(-0.5f * u * u);
+    return 0.5f * erfcf(z * 0.7071067811865476f);
 }
 
 template <bool FAST>
 __device__ __forceinline__ float act_value(float u, int act) {
     if (act == ACT_RELU) return u > 0.0f || u != u ? u : 0.0f;
     if (act == ACT_GELU) {
-        float cdf, pdf;
-        normal_cdf_pdf<FAST>(u, &cdf, &pdf);
-        return u * cdf;
+        // u Phi(u): u - u q above 0, u q below
+        float e;
+        const float q = normal_tail<FAST>(u, &e);
+        return __builtin_fmaf(-fabsf(u), q, u > 0.0f || u != u ? u : 0.0f);
     }
-    if (act == ACT_SILU) return u / (1.0f + (FAST ? __expf(-u) : expf(-u)));
+    if (act == ACT_SILU) {
+        if (FAST) return u * __builtin_amdgcn_rcpf(
+            1.0f + __builtin_amdgcn_exp2f(u * -1.44269504089f));
+        return u / (1.0f + expf(-u));
+    }
     return u;
 }
 
 template <bool FAST>
 __device__ __forceinline__ float act_slope(float u, int act) {
     if (act == ACT_GELU) {
-        float cdf, pdf;
-        normal_cdf_pdf<FAST>(u, &cdf, &pdf);
-        return cdf + u * pdf;
+        // Phi(u) + u phi(u), phi(u) = e / sqrt(2 pi)
+        float e;
+        const float q = normal_tail<FAST>(u, &e);
+        const float cdf = 0.5f + __builtin_copysignf(0.5f - q, u);
+        return __builtin_fmaf(u * e, 0.3989422804014327f, cdf);
     }
     if (act == ACT_SILU) {
-        const float s = 1.0f / (1.0f + (FAST ? __expf(-u) : expf(-u)));
-        return s * (1.0f + u * (1.0f - s));
+        const float s = FAST
+            ? __builtin_amdgcn_rcpf(
+                  1.0f + __builtin_amdgcn_exp2f(u * -1.44269504089f))
+            : 1.0f / (1.0f + expf(-u));
+        return s * __builtin_fmaf(u, 1.0f - s, 1.0f);
     }
     return 1.0f;
 }

@@ -52,13 +52,15 @@ __device__ __forceinline__ void dma16(u32x4 desc, unsigned lds, int voff,
                  : "scc");
 }
 
-// all but the last LATER copies into LDS and every read of LDS by this wave are
-// done, and the whole block has come here
-template <int LATER>
+// every copy into LDS and every read of LDS by this wave is done, and all WAVES
+// that share the tile have come here
+template <int WAVES>
 __device__ __forceinline__ void stage_wait() {
-    static_assert(LATER < 64, "vmcnt has 6 bits");
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier"
-                 :: "n"(LATER) : "memory");
+    if (WAVES == 1)
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    else
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier"
+                     ::: "memory");
 }
 
 __device__ __forceinline__ u32x4 buffer_desc(const void* p, long long bytes) {
@@ -84,7 +86,7 @@ __device__ __forceinline__ u32x4 buffer_desc(const void* p, long long bytes) {
 // across k: a stored row is one k.  16 bits: chunk c lies at c ^ 4 (k % 4), as
 //           the transposing read takes 32 bytes of 4 neighbouring k for each
 //           of 2 neighbouring blocks of 16 columns (rows of 128 bytes: c ^ 4
-//           (k / 2 % 2)); 32 bits: at c ^ 8 (k / 4 % 2), as the two halves of
+//           (k / 2 % 2), of 64 bytes: c); 32 bits: at c ^ 8 (k / 4 % 2), as the two halves of
 //           the lanes read 128 bytes each, 4 k apart.
 // Counters: conflicts fell from 97 to 1 of 100 read cycles at 8192^3.
 template <typename T, int ROWS, bool ALONG, int NWAVES>
@@ -96,11 +98,11 @@ struct Tile {
     static constexpr int CH = ROWB / 16;       // chunks in a stored row
     static constexpr int RPC = 1024 / ROWB;    // stored rows in one copy
     typedef typename Mfma<T>::V Frag;
-    static_assert(BYTES % (1024 * NWAVES) == 0 && CH >= 8, "tile");
+    static_assert(BYTES % (1024 * NWAVES) == 0 && CH >= 4, "tile");
 
     __device__ static __forceinline__ int swizzle(int r) {
         return ALONG ? (r >> 1) & 7
-             : SZ == 2 ? (CH >= 16 ? (r & 3) << 2 : (r & 2) << 1)
+             : SZ == 2 ? (CH >= 16 ? (r & 3) << 2 : CH == 8 ? (r & 2) << 1 : 0)
                        : CH >= 16 ? (r & 4) << 1 : 0;
     }
 
@@ -256,13 +258,15 @@ struct Gemm {
                                     const Operand& b_, int M_, int N_, int K_,
                                     int m0_, int n0_)
         : a(a_), b(b_), M(M_), N(N_), K(K_), m0(m0_), n0(n0_) {
-        tid = threadIdx.x;
+        // a wave by itself may be one of several in its block
+        tid = NW == 1 ? threadIdx.x & 63 : threadIdx.x;
         lane = tid & 63;
         wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         wm = wave / WN;
         wn = wave % WN;
         base = (lds_byte*)lds;
-        base_at = (unsigned)(unsigned long long)base;
+        base_at = __builtin_amdgcn_readfirstlane(
+            (unsigned)(unsigned long long)base);
         #pragma unroll
         for (int i = 0; i < TA::COPIES; ++i)
             va[i] = TA::source(wave, lane, i, (int)a.ld);
@@ -370,7 +374,7 @@ struct Gemm {
         if (mb)
             TB::mend(base + buf * STAGE + TA::BYTES, tid, THREADS, K - k,
                      N - n0, ob, at_b(k), (int)b.ld);
-        if (ma || mb) stage_wait<0>();
+        if (ma || mb) stage_wait<NW>();
     }
 
     // acc += a b over k0..k1; nobody uses the block's LDS
@@ -387,7 +391,7 @@ struct Gemm {
         constexpr int HALF = COPIES / 2, REST = COPIES - HALF;
         int buf = 0, k = k0;
         const bool one = k0 + BK >= k1;
-        stage_wait<0>();
+        stage_wait<NW>();
         if (one) {
             mend(k, k1, 0);
         } else {
@@ -401,7 +405,7 @@ struct Gemm {
             step<0, true, HALF, REST>(p, 1);
             step<1, true, 0, 0>(p, 2);
             step<0, true, 0, 0>(p, 3);
-            stage_wait<0>();
+            stage_wait<NW>();
             advance(buf);
             step<1, true, 0, HALF>(base + (buf ^ 1) * STAGE, 0);
         }
@@ -410,7 +414,7 @@ struct Gemm {
             step<0, true, HALF, REST>(p, 1);
             step<1, true, 0, 0>(p, 2);
             step<0, true, 0, 0>(p, 3);
-            stage_wait<0>();
+            stage_wait<NW>();
             buf ^= 1;
             mend(k + BK, k1, buf);
             step<1, true, 0, 0>(base + buf * STAGE, 0);

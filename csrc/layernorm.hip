@@ -319,12 +319,9 @@ at::Tensor row_sums(const Mat& p, at::ScalarType type) {
     return out;
 }
 
-// sums of `n` rows of partial sums, for linear.hip
-at::Tensor sum_partials(const at::Tensor& part, long long n, long long width,
-                        at::ScalarType type) {
-    auto out = at::empty({width}, part.options().dtype(type));
-    sum_columns(part, n, width, width, out, at::Tensor());
-    return out;
+// out = sum of the first n rows of partial sums, for linear.hip
+void sum_partials(const at::Tensor& part, long long n, at::Tensor& out) {
+    sum_columns(part, n, out.numel(), out.numel(), out, at::Tensor());
 }
 
 }  // namespace ffn

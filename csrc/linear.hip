@@ -16,14 +16,13 @@ namespace ffn {
     else { typedef float T; __VA_ARGS__; } \
 } while (0)
 
-at::Tensor sum_partials(const at::Tensor& part, long long n, long long width,
-                        at::ScalarType type);
+void sum_partials(const at::Tensor& part, long long n, at::Tensor& out);
 
 static hipStream_t stream_now() {
     return c10::hip::getCurrentHIPStream().stream();
 }
 
-// up to this many rows go to thin_kernel where it has a form for the operands
+// up to this many rows of an operand along k go to thin_kernel
 #define THIN_ROWS 64
 
 struct Plan { int tile, splits; };
@@ -125,17 +124,19 @@ static void product(at::ScalarType type, const Operand& a, const Operand& b,
     const bool quantises = EPI == EPI_FORWARD &&
                            (e.out8 || e.keep == KEEP_8BIT);
     if constexpr (AA) {
-        if (M <= THIN_ROWS && !quantises && !a.lo &&
-            (BA || type == at::kFloat)) {
+        if (M <= THIN_ROWS && !quantises && !a.lo) {
             const dim3 grid((unsigned)((N + 31) / 32),
                             (unsigned)((M + 31) / 32));
+            // 8 waves fill a unit's LDS, 4 leave room for a second block
+            const bool wide = (long long)grid.x * grid.y <= 256;
             FFN_TYPES(type,
-                if constexpr (BA || sizeof(T) == 4) {
-                    auto k = thin_kernel<T, BA, EPI>;
-                    hipLaunchKernelGGL(k, grid, THIN_WAVES * 64, 0,
-                                       stream_now(), a, b, (int)M, (int)N,
-                                       (int)K, e);
-                });
+                typedef Gemm<T, 32, 32, 1, 1, true, BA> G;
+                auto k = wide ? thin_kernel<T, BA, 8, EPI>
+                              : thin_kernel<T, BA, 4, EPI>;
+                const int waves = wide ? 8 : 4;
+                hipLaunchKernelGGL(k, grid, waves * 64, waves * G::LDS,
+                                   stream_now(), a, b, (int)M, (int)N,
+                                   (int)K, e));
             FFN_OK();
             *blocks = grid.y;
             return;
@@ -224,13 +225,30 @@ LinearOut linear_forward(const Mat& x, const Mat& w, const at::Tensor& bias,
     return o;
 }
 
-// rows of partial sums that any tile may write
-static at::Tensor empty_colsum(long long rows, long long dim,
-                               const at::Tensor& like) {
-    const int least = rows <= THIN_ROWS ? 16 : finish_rows(rows, dim);
-    return at::empty({(rows + least - 1) / least, dim},
-                     like.options().dtype(at::kFloat));
-}
+// Sums over the rows on their way: partial ones, one row of them for each block
+// of rows, or where one block has all rows (`one`) the result itself.
+struct Colsum {
+    at::Tensor out, part;
+    void aim(EpiArgs& e, long long rows, long long dim, const at::Tensor& bias,
+             bool one) {
+        out = at::empty({dim}, bias.options());
+        if (one) {
+            e.colsum = out.data_ptr();
+            e.colsum_out = bias.scalar_type() == at::kFloat ? COLSUM_FLOAT
+                                                            : COLSUM_T;
+            return;
+        }
+        // of 64 rows or more, or finish_kernel's
+        const int least = rows <= THIN_ROWS ? 16 : finish_rows(rows, dim);
+        part = at::empty({(rows + least - 1) / least, dim},
+                         bias.options().dtype(at::kFloat));
+        e.colsum = part.data_ptr();
+    }
+    at::Tensor join(long long blocks) {
+        if (part.defined()) sum_partials(part, blocks, out);
+        return out;
+    }
+};
 
 static Mat empty_grad(long long rows, long long dim, const at::Tensor& like,
                       bool split, const Kept& u) {
@@ -259,12 +277,9 @@ Mat through_act(const Mat& dy, int act, const Kept& u, const at::Tensor& bias,
     e.ld_out = p.ld;
     e.act = act;
     set_kept(e, u);
-    at::Tensor part;
-    if (bias.defined()) {
-        part = empty_colsum(p.rows, p.dim, p.t);
-        e.colsum = part.data_ptr<float>();
-    }
     const int rows = finish_rows(p.rows, p.dim);
+    Colsum sum;
+    if (bias.defined()) sum.aim(e, p.rows, p.dim, bias, p.rows <= rows);
     const dim3 grid((unsigned)((p.rows + rows - 1) / rows),
                     (unsigned)((p.dim + 127) / 128));
     FFN_TYPES(dy.t.scalar_type(),
@@ -272,8 +287,7 @@ Mat through_act(const Mat& dy, int act, const Kept& u, const at::Tensor& bias,
         hipLaunchKernelGGL(f, grid, 256, 0, stream_now(), (const T*)dy.t.data_ptr(), dy.ld, 1, rows,
                                           (int)p.rows, (int)p.dim, e));
     FFN_OK();
-    if (bias.defined())
-        *dbias = sum_partials(part, grid.x, p.dim, bias.scalar_type());
+    if (bias.defined()) *dbias = sum.join(grid.x);
     return p;
 }
 
@@ -298,16 +312,12 @@ Mat input_grad(const Mat& p, const Mat& w, int act, const Kept& u,
     e.ld_out = out.ld;
     e.act = act;
     set_kept(e, u);
-    at::Tensor part;
-    if (bias.defined()) {
-        part = empty_colsum(M, N, p.t);
-        e.colsum = part.data_ptr<float>();
-    }
+    Colsum sum;
+    if (bias.defined()) sum.aim(e, M, N, bias, M <= 16);
     long long blocks;
     product<true, false, EPI_GRAD>(p.t.scalar_type(), operand(p), operand(w),
                                    M, N, p.dim, e, p.t, &blocks);
-    if (bias.defined())
-        *dbias = sum_partials(part, blocks, N, bias.scalar_type());
+    if (bias.defined()) *dbias = sum.join(blocks);
     return out;
 }
 

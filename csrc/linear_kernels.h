@@ -19,18 +19,83 @@ struct EpiArgs {
     float* kept_scale;     // [M, N / 128]
     signed char* out8;     // 8-bit form of `out`, or null
     float* out8_scale;
-    float* colsum;         // EPI_GRAD: [row blocks, N] sums of `out`, or null
-    int act, keep, bias_f32, out_f32;
+    // EPI_GRAD: sums of `out` over the rows, or null: [row blocks, N] of float,
+    // or, where all rows are one block's, [N] of float or of T
+    void* colsum;
+    int act, keep, bias_f32, out_f32, colsum_out;
 };
+enum ColsumOut { COLSUM_FLOAT = 0, COLSUM_T = 1 };
 
 template <typename T> struct IsHalf { static constexpr bool value = true; };
 template <> struct IsHalf<float> { static constexpr bool value = false; };
 
+// What a chunk of 8 results needs from memory besides: the residual, or what is
+// kept of the value before the activation.  It is fetched long before its use.
+template <typename T> struct Extra {
+    typename Chunk<T>::V v;
+    u32x2 codes;
+    float scale;
+    unsigned bits;
+};
+
+__device__ __forceinline__ const float* scale_at(const float* scales,
+                                                 long long m, int n, int N) {
+    const int groups = (N + ACT8_GROUP - 1) / ACT8_GROUP;
+    return scales + m * groups + (n < N ? n / ACT8_GROUP : groups - 1);
+}
+
+// for row m, which is there, and columns from n on, which may not be
+template <typename T, int EPI>
+__device__ __forceinline__ void fetch_extra(Extra<T>& x, const EpiArgs& e,
+                                            long long m, int n, int N) {
+    if (EPI == EPI_FORWARD) {
+        if (e.res) x.v = fetch8((const T*)e.res + m * e.ld_res, n, N);
+    } else if (EPI == EPI_GRAD) {
+        if (e.keep == KEEP_FULL) {
+            x.v = fetch8((const T*)e.kept + m * N, n, N);
+        } else if (e.keep == KEEP_8BIT) {
+            const signed char* p = (const signed char*)e.kept + m * N;
+            if (N >= 8) {
+                x.codes = __builtin_bit_cast(u32x2,
+                    *reinterpret_cast<const i8x8*>(
+                        p + (n < N - 8 ? n : N - 8)));
+            } else {
+                i8x8 c;
+                #pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    c[i] = i < N ? p[i] : (signed char)0;
+                x.codes = __builtin_bit_cast(u32x2, c);
+            }
+            x.scale = *scale_at(e.kept_scale, m, n, N);
+        } else if (e.keep == KEEP_BITS) {
+            const int bytes = (N + 7) >> 3, at = n >> 3;
+            x.bits = ((const unsigned char*)e.kept)
+                [m * bytes + (at < bytes ? at : bytes - 1)];
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void load_bias(const EpiArgs& e, int n, int N,
+                                          float* b) {
+    if (!e.bias) {
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) b[i] = 0.0f;
+    } else if (e.bias_f32) {
+        load8((const float*)e.bias + n, N - n, b);
+    } else {
+        load8((const T*)e.bias + n, N - n, b);
+    }
+}
+
 // 8 neighbouring results of row m from column n on; `left` of them are there
-// (0 or less: none).  All 16 lanes of a group of 128 columns come together.
+// (0 or less: none), all 8 where it is `whole` (the same for all lanes).  All
+// 16 lanes of a group of 128 columns come together.
 template <typename T, int EPI>
 __device__ __forceinline__ void finish8(float* v, long long m, int n, int left,
-                                        int N, const EpiArgs& e, float* sums) {
+                                        int N, bool whole, const EpiArgs& e,
+                                        const float* bias, const Extra<T>& x,
+                                        float* sums) {
     constexpr bool FAST = IsHalf<T>::value;
     const bool on = left > 0;
     if (EPI == EPI_PLAIN) {
@@ -40,30 +105,29 @@ __device__ __forceinline__ void finish8(float* v, long long m, int n, int left,
         return;
     }
     if (EPI == EPI_GRAD) {
-        if (!on) return;
         // what comes from the layer above is of type T: rounded as such
         #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = (float)(T)v[i];
         if (e.keep == KEEP_BITS) {
-            const unsigned bits = ((const unsigned char*)e.kept)
-                [m * ((N + 7) >> 3) + (n >> 3)];
             #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (!(bits >> i & 1)) v[i] = 0.0f;
+                if (!(x.bits >> i & 1)) v[i] = 0.0f;
         } else if (e.keep != KEEP_NONE) {
             float u[8];
-            if (e.keep == KEEP_8BIT)
-                load8_codes((const signed char*)e.kept + m * N + n, left,
-                            e.kept_scale[m * ((N + ACT8_GROUP - 1) /
-                                              ACT8_GROUP) + n / ACT8_GROUP],
-                            u);
-            else
-                load8((const T*)e.kept + m * N + n, left, u);
+            if (e.keep == KEEP_8BIT) {
+                unpack8(__builtin_bit_cast(i8x8, x.codes), n, N, whole, u);
+                #pragma unroll
+                for (int i = 0; i < 8; ++i) u[i] *= x.scale;
+            } else {
+                unpack8(x.v, n, N, whole, u);
+            }
             #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] *= act_slope<FAST>(u[i], e.act);
         }
+        if (!on) return;
         #pragma unroll
-        for (int i = 0; i < 8; ++i) sums[i] += i < left ? v[i] : 0.0f;
+        for (int i = 0; i < 8; ++i)
+            sums[i] += whole || i < left ? v[i] : 0.0f;
         store8((T*)e.out + m * e.ld_out + n, left, v);
         if (e.out_lo) {
             #pragma unroll
@@ -75,15 +139,11 @@ __device__ __forceinline__ void finish8(float* v, long long m, int n, int left,
         }
         return;
     }
-    if (on && e.bias) {
-        float b[8];
-        if (e.bias_f32) load8((const float*)e.bias + n, left, b);
-        else load8((const T*)e.bias + n, left, b);
-        #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += b[i];
-    }
     #pragma unroll
-    for (int i = 0; i < 8; ++i) if (i >= left) v[i] = 0.0f;
+    for (int i = 0; i < 8; ++i) {
+        v[i] += bias[i];
+        if (!whole && i >= left) v[i] = 0.0f;
+    }
     if (e.keep == KEEP_BITS) {
         unsigned bits = 0;
         #pragma unroll
@@ -107,9 +167,9 @@ __device__ __forceinline__ void finish8(float* v, long long m, int n, int left,
         #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = act_value<FAST>(v[i], e.act);
     }
-    if (on && e.res) {
+    if (e.res) {
         float r[8];
-        load8((const T*)e.res + m * e.ld_res + n, left, r);
+        unpack8(x.v, n, N, whole, r);
         #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] += r[i];
     }
@@ -117,7 +177,7 @@ __device__ __forceinline__ void finish8(float* v, long long m, int n, int left,
     if (e.out8) {
         #pragma unroll
         for (int i = 0; i < 8; ++i)
-            v[i] = i < left ? (float)(T)v[i] : 0.0f;
+            v[i] = whole || i < left ? (float)(T)v[i] : 0.0f;
         const float a = max16(max8(v));
         const Act8Scale s = act8_scale(a, a < __builtin_inff());
         if (on) {
@@ -127,6 +187,14 @@ __device__ __forceinline__ void finish8(float* v, long long m, int n, int left,
                              n / ACT8_GROUP] = s.scale;
         }
     }
+}
+
+// column sums of a block of rows: one of several, to be joined, or the result
+template <typename T>
+__device__ __forceinline__ void put_colsum(const EpiArgs& e, long long block,
+                                           int n, int N, float t) {
+    if (e.colsum_out == COLSUM_T) ((T*)e.colsum)[n] = (T)t;
+    else ((float*)e.colsum)[block * N + n] = t;
 }
 
 // One block, one tile of C; blockIdx.y is the part of k.  With `part` the
@@ -150,34 +218,57 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(
     g.run(k0, k1);
     if (a.lo) {
         g.a.p = a.lo;
-        stage_wait<0>();
+        stage_wait<G::NW>();
         g.run(k0, k1);
     }
 
     constexpr int CH = BN / 8;             // chunks of 8 columns
     constexpr int RS = G::THREADS / CH;    // rows a round
+    constexpr int ROUNDS = WM * 32 / RS;
     const int c = threadIdx.x % CH, r0 = threadIdx.x / CH;
     const int n = n0 + 8 * c, left = N - n;
-    float sums[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    #pragma unroll
+    const bool whole = n0 + BN <= N;
+    float sums[8] = {0, 0, 0, 0, 0, 0, 0, 0}, bias[8];
+    if (EPI == EPI_FORWARD && !part) load_bias<T>(e, n, N, bias);
+    auto row_of = [&](int i, int round) {
+        const int r = r0 + round * RS;
+        return m0 + ((r >> 5) * G::TM + i) * 32 + (r & 31);
+    };
+    // Each pass's extras are on their way while the pass before is written, or a
+    // pass would wait for memory four times.  The passes share their code: what
+    // they do is long, and instructions come through a cache too.
+    Extra<T> x[ROUNDS];
+    auto fetch = [&](int i, int q) {
+        const int m = row_of(i, q);
+        fetch_extra<T, EPI>(x[q], e, m < M ? m : M - 1, n, N);
+    };
+    if (!part) {
+        #pragma unroll
+        for (int q = 0; q < ROUNDS; ++q) fetch(0, q);
+    }
+    #pragma unroll 1
     for (int i = 0; i < G::TM; ++i) {
         __syncthreads();
-        g.stage_out(lds, i);
+        #pragma unroll
+        for (int j = 0; j < G::TM; ++j)
+            if (i == j) g.stage_out(lds, j);
         __syncthreads();
-        for (int r = r0; r < WM * 32; r += RS) {
+        #pragma unroll
+        for (int q = 0; q < ROUNDS; ++q) {
             const float* s = reinterpret_cast<const float*>(lds) +
-                             r * G::OUT_LD + 8 * c;
+                             (r0 + q * RS) * G::OUT_LD + 8 * c;
             float v[8];
             #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = s[j];
-            const int m = m0 + ((r >> 5) * G::TM + i) * 32 + (r & 31);
+            const int m = row_of(i, q);
             const int here = m < M ? left : 0;
             if (part) {
                 if (here > 0)
                     store8(part + ((long long)blockIdx.y * M + m) * ld_part +
                            n, here, v);
             } else {
-                finish8<T, EPI>(v, m, n, here, N, e, sums);
+                finish8<T, EPI>(v, m, n, here, N, whole, e, bias, x[q], sums);
+                if (i + 1 < G::TM) fetch(i + 1, q);
             }
         }
     }
@@ -190,91 +281,64 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(
         for (int j = threadIdx.x; j < BN; j += G::THREADS) {
             float t = 0.0f;
             for (int r = 0; r < RS; ++r) t += all[r * BN + j];
-            if (n0 + j < N) e.colsum[(long long)bm * N + n0 + j] = t;
+            if (n0 + j < N) put_colsum<T>(e, bm, n0 + j, N, t);
         }
     }
 }
 
-// Few rows: 32 x 32 results a block, k shared out among its 8 waves.  The
-// fragments come straight from memory, 16 bytes a lane along k: there is nothing
-// to share, and no barrier before the end.  What bounds it is the weight's way
-// from memory.  BA false (32 bits only): a lane's 4 values of B lie across k.
-#define THIN_WAVES 8
-template <typename T, bool BA, int EPI>
-__global__ __launch_bounds__(THIN_WAVES * 64) void thin_kernel(
+// Few rows: 32 x 32 results a block, k shared out among its KW waves.  Each wave
+// has stages of its own and waits for nobody before the end.  What bounds it is
+// the weight's way from memory, 8 KB a wave under way.  (Fragments straight from
+// memory, without LDS, took 17 us for 20 x 1500 by 10000: a load of 16 bytes from
+// each of 32 rows is 64 requests to the cache, a copy of 8 rows 16 at most.)
+template <typename T, bool BA, int KW, int EPI>
+__global__ __launch_bounds__(KW * 64) void thin_kernel(
         Operand a, Operand b, int M, int N, int K, EpiArgs e) {
-    static_assert(BA || sizeof(T) == 4, "across k needs 32 bits");
-    constexpr int E = 16 / sizeof(T), U = 2 * E, LD = 36;
-    typedef T V __attribute__((ext_vector_type(E), aligned(sizeof(T))));
-    __shared__ float part[THIN_WAVES][32][LD];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int row = lane & 31, off = E * (lane >> 5);
+    typedef Gemm<T, 32, 32, 1, 1, true, BA> G;
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+    const int wave = threadIdx.x >> 6;
     const int m0 = blockIdx.y * 32, n0 = blockIdx.x * 32;
-    // rows that are not there: the last one's values, for results not written
-    const long long ma = m0 + row < M ? m0 + row : M - 1;
-    const long long nb = n0 + row < N ? n0 + row : N - 1;
-    const T* pa = (const T*)a.p + ma * a.ld + off;
-    const T* pb = (const T*)b.p + (BA ? nb * b.ld + off : off * b.ld + nb);
-    const int steps = (K + U - 1) / U;
-    const int per = (steps + THIN_WAVES - 1) / THIN_WAVES;
-    const int s0 = wave * per, s1 = s0 + per < steps ? s0 + per : steps;
-    const int whole = K / U < s1 ? K / U : s1;
-    f32x16 acc;
-    #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
-    auto step = [&](int s, bool all) {
-        typename Mfma<T>::V x, y;
-        const int k = s * U;
-        if (all) {
-            x = *reinterpret_cast<const V*>(pa + k);
-        } else {
-            #pragma unroll
-            for (int i = 0; i < E; ++i)
-                x[i] = k + off + i < K ? pa[k + i] : (T)0.0f;
-        }
-        if (BA && all) {
-            y = *reinterpret_cast<const V*>(pb + k);
-        } else {
-            #pragma unroll
-            for (int i = 0; i < E; ++i)
-                y[i] = all || k + off + i < K
-                    ? pb[BA ? k + i : (long long)(k + i) * b.ld] : (T)0.0f;
-        }
-        acc = Mfma<T>::go(y, x, acc);
-    };
-    #pragma unroll 6
-    for (int s = s0; s < whole; ++s) step(s, true);
-    if (s0 < s1 && whole < s1) step(whole, false);
-    #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-        f32x4 v;
-        #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = acc[4 * g + i];
-        *reinterpret_cast<f32x4*>(&part[wave][row][8 * g + 4 * (lane >> 5)]) = v;
-    }
-    __syncthreads();
+    const int steps = (K + G::BK - 1) / G::BK;
+    const int per = (steps + KW - 1) / KW * G::BK;
+    const int k0 = __builtin_amdgcn_readfirstlane(wave * per);
+    const int k1 = K - k0 < per ? K : k0 + per;
+    unsigned char* own = lds + wave * G::LDS;
+    G g(own, a, b, M, N, K, m0, n0);
+    if (k0 < k1) g.run(k0, k1);
     const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 8;
-    float sums[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    const bool whole = n0 + 32 <= N;
+    Extra<T> extra;
+    float bias[8], sums[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (threadIdx.x < 128) {
+        fetch_extra<T, EPI>(extra, e, m0 + r < M ? m0 + r : M - 1, n0 + c, N);
+        if (EPI == EPI_FORWARD) load_bias<T>(e, n0 + c, N, bias);
+    }
+    g.stage_out(own, 0);
+    __syncthreads();
     if (threadIdx.x < 128) {
         float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         #pragma unroll
-        for (int w = 0; w < THIN_WAVES; ++w)
+        for (int w = 0; w < KW; ++w) {
+            const float* p = reinterpret_cast<const float*>(
+                lds + w * G::LDS) + r * G::OUT_LD + c;
             #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] += part[w][r][c + i];
-        finish8<T, EPI>(v, m0 + r, n0 + c, m0 + r < M ? N - n0 - c : 0, N, e,
-                        sums);
+            for (int i = 0; i < 8; ++i) v[i] += p[i];
+        }
+        finish8<T, EPI>(v, m0 + r, n0 + c, m0 + r < M ? N - n0 - c : 0, N,
+                        whole, e, bias, extra, sums);
     }
     if (EPI == EPI_GRAD && e.colsum) {
+        float* all = reinterpret_cast<float*>(lds);
         __syncthreads();
         if (threadIdx.x < 128) {
             #pragma unroll
-            for (int i = 0; i < 8; ++i) part[0][r][c + i] = sums[i];
+            for (int i = 0; i < 8; ++i) all[r * 32 + c + i] = sums[i];
         }
         __syncthreads();
         if (threadIdx.x < 32 && n0 + threadIdx.x < N) {
             float t = 0.0f;
-            for (int i = 0; i < 32; ++i) t += part[0][i][threadIdx.x];
-            e.colsum[(long long)blockIdx.y * N + n0 + threadIdx.x] = t;
+            for (int i = 0; i < 32; ++i) t += all[i * 32 + threadIdx.x];
+            put_colsum<T>(e, blockIdx.y, n0 + threadIdx.x, N, t);
         }
     }
 }
@@ -290,21 +354,27 @@ __global__ __launch_bounds__(256) void finish_kernel(
     __shared__ float all[16 * 128];
     const int c = threadIdx.x & 15, r0 = threadIdx.x >> 4;
     const int n = blockIdx.y * 128 + 8 * c, left = N - n;
-    float sums[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    const bool whole = (int)(blockIdx.y + 1) * 128 <= N;
+    float sums[8] = {0, 0, 0, 0, 0, 0, 0, 0}, bias[8];
+    if (EPI == EPI_FORWARD) load_bias<T>(e, n, N, bias);
     for (int r = r0; r < rows; r += 16) {
         const long long m = (long long)blockIdx.x * rows + r;
+        const long long there = m < M ? m : M - 1;
         const int here = m < M ? left : 0;
-        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (here > 0) {
-            #pragma unroll 4
-            for (int s = 0; s < splits; ++s) {
-                float w[8];
-                load8(part + ((long long)s * M + m) * ld_part + n, here, w);
-                #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] += w[j];
-            }
+        Extra<T> x;
+        fetch_extra<T, EPI>(x, e, there, n, N);
+        float v[8];
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+        #pragma unroll 4
+        for (int s = 0; s < splits; ++s) {
+            float w[8];
+            unpack8(fetch8(part + ((long long)s * M + there) * ld_part, n, N),
+                    n, N, whole, w);
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += w[j];
         }
-        finish8<T, EPI>(v, m, n, here, N, e, sums);
+        finish8<T, EPI>(v, m, n, here, N, whole, e, bias, x, sums);
     }
     if (EPI == EPI_GRAD && e.colsum) {
         #pragma unroll
@@ -314,7 +384,7 @@ __global__ __launch_bounds__(256) void finish_kernel(
             float t = 0.0f;
             for (int r = 0; r < 16; ++r) t += all[r * 128 + threadIdx.x];
             const int col = blockIdx.y * 128 + threadIdx.x;
-            if (col < N) e.colsum[(long long)blockIdx.x * N + col] = t;
+            if (col < N) put_colsum<T>(e, blockIdx.x, col, N, t);
         }
     }
 }
