@@ -66,26 +66,43 @@ __device__ __forceinline__ typename Chunk<T>::V fetch8(const T* row, int c,
     return v;
 }
 
-// columns that are not there become 0.  `whole`: no lane's chunk ends past the
-// row (the same for all lanes).
-__device__ __forceinline__ void settle8(int c, int dim, bool whole, float* v) {
-    if (whole) return;
-    const int by = dim >= 8 && c > dim - 8 ? c - (dim - 8) : 0;
+// What fetch8 brought, with the columns where they belong and zeros in those that
+// are not there: shifted down as a whole, and only where a lane's chunk ends past
+// the row (done on single values by all lanes, this took as long as the rest of
+// the norm).
+template <typename V>
+__device__ __forceinline__ V settle8(V raw, int c, int dim) {
+    constexpr int W = sizeof(V) / 4, SZ = sizeof(V) / 8;
+    const int over = dim >= 8 ? c - (dim - 8) : c;
+    if (!__any(over > 0)) return raw;
+    const int by = over <= 0 ? 0 : over < 8 && dim >= 8 ? over * SZ : 8 * SZ;
+    union { V v; unsigned d[W]; } u;
+    u.v = raw;
     #pragma unroll
-    for (int b = 1; b < 8; b *= 2)
+    for (int b = SZ; b < 4; b *= 2)
         #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] = by & b ? (i + b < 8 ? v[i + b] : 0.0f) : v[i];
+        for (int i = 0; i < W; ++i)
+            u.d[i] = by & b
+                ? __builtin_amdgcn_alignbyte(i + 1 < W ? u.d[i + 1] : 0u,
+                                             u.d[i], b)
+                : u.d[i];
     #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < dim ? v[i] : 0.0f;
+    for (int b = 4; b < 8 * SZ; b *= 2)
+        #pragma unroll
+        for (int i = 0; i < W; ++i)
+            u.d[i] = by & b ? (i + b / 4 < W ? u.d[i + b / 4] : 0u) : u.d[i];
+    #pragma unroll
+    for (int i = 0; i < W; ++i) u.d[i] = by == 8 * SZ ? 0u : u.d[i];
+    return u.v;
 }
 
+// `whole`: no lane's chunk ends past the row (the same for all lanes)
 template <typename V>
 __device__ __forceinline__ void unpack8(V raw, int c, int dim, bool whole,
                                         float* v) {
+    if (!whole) raw = settle8(raw, c, dim);
     #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = (float)raw[i];
-    settle8(c, dim, whole, v);
 }
 
 template <typename T>
@@ -121,40 +138,61 @@ __device__ __forceinline__ void load8_codes(const signed char* p, int left,
 // all of it reads as NaN, so a broken activation shows in the gradients.
 struct Act8Scale { float by, scale; };
 
-__device__ __forceinline__ Act8Scale act8_scale(float a, bool finite) {
+// the group's largest magnitude comes as the bits of |x|, which order as the
+// values do, infinities and then NaN at the end
+__device__ __forceinline__ Act8Scale act8_scale(unsigned bits) {
     Act8Scale s;
-    const bool some = a >= ACT8_LEAST;
-    s.by = some && finite ? 127.0f / a : 0.0f;
+    const float a = __uint_as_float(bits);
+    const bool finite = bits < 0x7f800000u;
+    const bool some = finite && a >= ACT8_LEAST;
+    s.by = some ? 127.0f / a : 0.0f;
     s.scale = !finite ? __builtin_nanf("")
                       : some ? a * (1.0f / 127.0f) : 0.0f;
     return s;
 }
 
-// max |x| over 8 values; `finite` falls where one is an infinity or NaN
-__device__ __forceinline__ float max8(const float* v) {
-    // fmax drops NaN, so NaN is carried as an infinity
-    float a = 0.0f;
+// largest magnitude of 8 values, as bits
+__device__ __forceinline__ unsigned max8(const float* v) {
+    unsigned a = 0;
     #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float m = fabsf(v[i]);
-        a = fmaxf(a, m == m ? m : __builtin_inff());
+        const unsigned m = __float_as_uint(v[i]) & 0x7fffffffu;
+        a = a > m ? a : m;
     }
     return a;
 }
 
+// rint by adding 1.5 * 2^23, which leaves the integer in the low bits: the same
+// for products up to 127 (1 + 2^-23); the bytes are then picked, four to a word
 __device__ __forceinline__ void store8_codes(signed char* p, int left,
                                              const float* v, float by) {
-    i8x8 c;
+    // the product rounds by itself, by definition: no fma
+    #pragma clang fp contract(off)
+    unsigned q[8], w[2];
     #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        // by is 0 in a group of zeros and in one that is not finite
-        c[i] = by == 0.0f ? (signed char)0
-                          : (signed char)(int)rintf(v[i] * by);
+    for (int i = 0; i < 8; ++i) {
+        const float x = v[i] * by;
+        q[i] = __float_as_uint(x + 12582912.0f);
+    }
+    #pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const unsigned lo = __builtin_amdgcn_perm(q[4 * h + 1], q[4 * h],
+                                                  0x0c0c0400u);
+        const unsigned hi = __builtin_amdgcn_perm(q[4 * h + 3], q[4 * h + 2],
+                                                  0x04000c0cu);
+        // groups of zeros, and those that are not finite
+        w[h] = by == 0.0f ? 0u : lo | hi;
+    }
     if (left >= 8) {
-        *reinterpret_cast<i8x8*>(p) = c;
+        typedef unsigned V __attribute__((ext_vector_type(2), aligned(1)));
+        V c;
+        c[0] = w[0];
+        c[1] = w[1];
+        *reinterpret_cast<V*>(p) = c;
     } else {
         #pragma unroll
-        for (int i = 0; i < 8; ++i) if (i < left) p[i] = c[i];
+        for (int i = 0; i < 8; ++i)
+            if (i < left) p[i] = (signed char)(w[i >> 2] >> (8 * (i & 3)));
     }
 }
 
@@ -168,11 +206,16 @@ __device__ __forceinline__ float moved(float v) {
 
 // max over 16 neighbouring lanes (one group of 128 values, 8 a lane): each lane
 // takes in the one 8, 4, 2 and 1 lanes round
-__device__ __forceinline__ float max16(float a) {
-    a = fmaxf(a, moved<0x128, 0xf>(a));
-    a = fmaxf(a, moved<0x124, 0xf>(a));
-    a = fmaxf(a, moved<0x122, 0xf>(a));
-    return fmaxf(a, moved<0x121, 0xf>(a));
+template <int CTRL>
+__device__ __forceinline__ unsigned max_moved(unsigned a) {
+    const unsigned b = __builtin_amdgcn_update_dpp(0, a, CTRL, 0xf, 0xf, true);
+    return a > b ? a : b;
+}
+__device__ __forceinline__ unsigned max16(unsigned a) {
+    a = max_moved<0x128>(a);
+    a = max_moved<0x124>(a);
+    a = max_moved<0x122>(a);
+    return max_moved<0x121>(a);
 }
 
 // sum over the wave, the same in all lanes: over 16 lanes from the left, then

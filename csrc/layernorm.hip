@@ -69,7 +69,7 @@ Packed pack(const Mat& x) {
     Packed p = empty_packed(x.rows, x.dim, x.t);
     const long long groups = x.rows * groups_in(x.dim);
     if (!groups) return p;
-    const int grid = (int)std::min<long long>((groups + 63) / 64, 256 * 16);
+    const int grid = (int)std::min<long long>((groups + 31) / 32, 256 * 64);
     FFN_TYPES(x.t.scalar_type(), FFN_COUNT(groups,
         auto k = act8_pack_kernel<T, I>;
         hipLaunchKernelGGL(k, grid, 256, 0, stream_now(),
@@ -105,7 +105,9 @@ Mat unpack(const at::Tensor& codes, const at::Tensor& scales,
     }
     const long long n = rows * ((dim + 7) / 8);
     if (!n) return out;
-    const int grid = (int)std::min<long long>((n + 1023) / 1024, 256 * 16);
+    TORCH_CHECK(n < (1LL << 38), "8-bit form of ", rows, " x ", dim,
+                " is too large");
+    const unsigned grid = (unsigned)((n + 255) / 256);
     FFN_TYPES(type, FFN_COUNT(n,
         auto k = act8_unpack_kernel<T, I>;
         hipLaunchKernelGGL(k, grid, 256, 0, stream_now(),
@@ -118,15 +120,19 @@ Mat unpack(const at::Tensor& codes, const at::Tensor& scales,
 
 // team of threads a row, chunks of 8 a thread.  Forward: as few threads as hold
 // the row in 4 chunks each, so that a row of up to 2048 values needs no barrier.
-// Backward: as many threads as there are chunks, up to 1024, since a chunk takes
-// 32 registers there.  17920 x 1500 in bf16, x in 8 bits: 64 threads with 3
-// chunks 68 us (194 registers, two waves a unit), 256 with one BWD_US us.
+// Backward: about as many threads as there are chunks, up to 1024, since a chunk
+// takes 32 registers and both kernels are bound by instructions: 17920 x 1500 in
+// bf16, x in 8 bits, 64 threads with 3 chunks 68 us (194 registers, two waves a
+// unit), 256 with one 42.
 #define NORM_BACKWARD_SHAPES(dim, WIDE, GO) do { \
     const long long chunks = ((dim) + 7) / 8; \
     if (chunks <= 64) GO(64, 1); \
     else if (chunks <= 128) GO(128, 1); \
+    else if (chunks <= 192) GO(192, 1); \
     else if (chunks <= 256) GO(256, 1); \
+    else if (chunks <= 384) GO(384, 1); \
     else if (chunks <= 512) GO(512, 1); \
+    else if (chunks <= 768) GO(768, 1); \
     else if (chunks <= 1024) GO(1024, 1); \
     else if (chunks <= 2048) GO(1024, 2); \
     else if (chunks <= 4096) GO(1024, 4); \
@@ -263,7 +269,7 @@ NormGrads norm_backward(const Mat& x, const Packed& x8, const Mat& dy,
     #define GO(NT, R) do { \
         const int teams = NT == 64 ? 4 : 1, threads = NT == 64 ? 256 : NT; \
         blocks = std::min<long long>((rows + teams - 1) / teams, \
-                                     NT <= 256 ? 1024 : NT == 512 ? 512 : 256); \
+                                     NT <= 256 ? 1024 : NT <= 512 ? 512 : 256); \
         if (params) { \
             part = at::empty({blocks, 2, dim}, f32); \
             a.part = part.data_ptr<float>(); \

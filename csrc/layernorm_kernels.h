@@ -60,8 +60,7 @@ __device__ __forceinline__ void load_param(const void* p, int p32, int c,
 __device__ __forceinline__ void keep8(signed char* codes, float* scales,
                                       long long row, int c, int left, int dim,
                                       const float* v) {
-    const float a = max16(max8(v));
-    const Act8Scale s = act8_scale(a, a < __builtin_inff());
+    const Act8Scale s = act8_scale(max16(max8(v)));
     if (left > 0) {
         store8_codes(codes + row * dim + c, left, v, s.by);
         if (c % ACT8_GROUP == 0)
@@ -107,19 +106,27 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_forward_kernel(
             raw[i] = fetch8(x, (i * NT + t) * 8, p.dim);
         #pragma unroll
         for (int i = 0; i < R; ++i) {
-            unpack8(raw[i], (i * NT + t) * 8, p.dim,
-                    (i + 1) * NT * 8 <= p.dim, v[i]);
+            const int c = (i * NT + t) * 8;
+            unpack8(raw[i], c, p.dim, (i + 1) * NT * 8 <= p.dim, v[i]);
             #pragma unroll
             for (int j = 0; j < 8; ++j) s += v[i][j];
+            if (p.x8)
+                keep8(p.x8, p.x8_scale, row, c, p.dim - c, p.dim, v[i]);
         }
         team_sum2<NT>(s, none, slots[0]);
         float mean = s / n, more = 0.0f;
         #pragma unroll
         for (int i = 0; i < R; ++i) {
             const int left = p.dim - (i * NT + t) * 8;
+            if ((i + 1) * NT * 8 > p.dim) {
+                // columns that are not there count nothing
+                #pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    v[i][j] = j < left ? v[i][j] : mean;
+            }
             #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float d = j < left ? v[i][j] - mean : 0.0f;
+                const float d = v[i][j] - mean;
                 q += d * d;
                 more += d;
             }
@@ -130,7 +137,6 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_forward_kernel(
         #pragma unroll
         for (int i = 0; i < R; ++i) {
             const int c = (i * NT + t) * 8, left = p.dim - c;
-            if (p.x8) keep8(p.x8, p.x8_scale, row, c, left, p.dim, v[i]);
             #pragma unroll
             for (int j = 0; j < 8; ++j)
                 v[i][j] = (v[i][j] - mean) * rstd * g[i][j] + b[i][j];
@@ -175,7 +181,7 @@ template <typename T, bool X8> struct KeptRaw {
                                            float* v) const {
         unpack8(raw, c, dim, whole, v);
     }
-    __device__ __forceinline__ void renew() { asm volatile("" : "+v"(raw)); }
+    __device__ __forceinline__ float by(float rstd) const { return rstd; }
 };
 template <typename T> struct KeptRaw<T, true> {
     u32x2 raw;
@@ -200,10 +206,11 @@ template <typename T> struct KeptRaw<T, true> {
     __device__ __forceinline__ void unpack(int c, int dim, bool whole,
                                            float* v) const {
         unpack8(__builtin_bit_cast(i8x8, raw), c, dim, whole, v);
-        #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= scale;
     }
-    __device__ __forceinline__ void renew() { asm volatile("" : "+v"(raw)); }
+    // what a code is multiplied by
+    __device__ __forceinline__ float by(float rstd) const {
+        return scale * rstd;
+    }
 };
 
 template <typename T>
@@ -250,51 +257,46 @@ __global__ __launch_bounds__(NT < 128 ? 256 : NT) void norm_backward_kernel(
             rh[i].fetch(p, row, c);
             rd[i] = fetch8((const T*)p.dy + row * p.ld_dy, c, p.dim);
         }
-        // xh and dy of a chunk; columns that are not there have dy = 0
-        auto values = [&](int i, float* h, float* d) {
-            const int c = (i * NT + t) * 8;
-            const bool whole = (i + 1) * NT * 8 <= p.dim;
-            rh[i].unpack(c, p.dim, whole, h);
-            unpack8(rd[i], c, p.dim, whole, d);
-            #pragma unroll
-            for (int j = 0; j < 8; ++j) h[j] = (h[j] - mean) * rstd;
-        };
+        // xh = x rstd - mean rstd, a code times its scale and rstd; columns that
+        // are not there have dy = 0
+        float h[R][8], d[R][8];
+        const float shift = -mean * rstd;
         #pragma unroll
         for (int i = 0; i < R; ++i) {
-            float h[8], d[8];
-            values(i, h, d);
+            const int c = (i * NT + t) * 8;
+            const bool whole = (i + 1) * NT * 8 <= p.dim;
+            rh[i].unpack(c, p.dim, whole, h[i]);
+            unpack8(rd[i], c, p.dim, whole, d[i]);
+            const float by = rh[i].by(rstd);
             #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                sg[i][j] += d[j] * h[j];
-                sb[i][j] += d[j];
-                d[j] *= g[i][j];
-                s1 += d[j];
-                s2 += d[j] * h[j];
+                h[i][j] = __builtin_fmaf(h[i][j], by, shift);
+                sg[i][j] = __builtin_fmaf(d[i][j], h[i][j], sg[i][j]);
+                sb[i][j] += d[i][j];
+                d[i][j] *= g[i][j];
+                s1 += d[i][j];
+                s2 = __builtin_fmaf(d[i][j], h[i][j], s2);
             }
         }
         if (!p.dx) continue;
         team_sum2<NT>(s1, s2, slots[turn]);
-        s1 *= inv;
-        s2 *= inv;
+        s1 *= -inv * rstd;
+        s2 *= -inv * rstd;
         #pragma unroll
         for (int i = 0; i < R; ++i) {
-            // unpacked anew: kept as 32 bits, the row would take the registers
-            // of a second wave
-            asm volatile("" : "+v"(rd[i]));
-            rh[i].renew();
             const int c = (i * NT + t) * 8, left = p.dim - c;
-            float h[8], d[8], a[8];
-            values(i, h, d);
+            float a[8];
             if (p.add)
                 unpack8(fetch8((const T*)p.add + row * p.ld_add, c, p.dim), c,
                         p.dim, (i + 1) * NT * 8 <= p.dim, a);
             #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float v = rstd * (d[j] * g[i][j] - s1 - h[j] * s2);
-                d[j] = p.add ? v + a[j] : v;
+                const float v = __builtin_fmaf(
+                    h[i][j], s2, __builtin_fmaf(d[i][j], rstd, s1));
+                d[i][j] = p.add ? v + a[j] : v;
             }
             if (left > 0)
-                store8((T*)p.dx + (long long)row * p.dim + c, left, d);
+                store8((T*)p.dx + (long long)row * p.dim + c, left, d[i]);
         }
     }
     if (!p.part) return;
@@ -424,7 +426,7 @@ __global__ __launch_bounds__(256) void row_sum_kernel(NormGradArgs p,
     float sg[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sb[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (left > 0) {
         const bool whole = (blockIdx.x + 1) * 256 <= p.dim;
-        #pragma unroll 8
+        #pragma unroll 4
         for (int row = first + r0; row < last; row += 8) {
             float d[8], h[8];
             unpack8(fetch8((const T*)p.dy + row * p.ld_dy, c, p.dim), c, p.dim,
@@ -480,12 +482,13 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(
 
 // ---- the 8-bit form by itself ------------------------------------------------------
 // A group of 128 values for each 16 lanes, GROUPS of them at a time; I is the
-// type that counts them.
+// type that counts them.  17920 x 6000 in bf16, us: one group 66, two 64, four
+// 66, and 74 with a quarter of the blocks.
 template <typename T, typename I>
 __global__ __launch_bounds__(256) void act8_pack_kernel(
         const T* x, long long ld, I rows, int dim, signed char* codes,
         float* scales) {
-    constexpr int GROUPS = 4;
+    constexpr int GROUPS = 2;
     const I ng = groups_of(dim), groups = rows * ng;
     const int t = threadIdx.x >> 4, o = (threadIdx.x & 15) * 8;
     // all lanes of a wave go round as often, for max16
@@ -511,44 +514,29 @@ __global__ __launch_bounds__(256) void act8_pack_kernel(
     }
 }
 
-// Values of 8 bits to 16 or 32, rows ld apart.
+// Values of 8 bits to 16 or 32, rows ld apart, a chunk of 8 a thread: 17920 x 6000
+// to fp32 93 us; with two to eight chunks a thread 115 to 137.
 template <typename O, typename I>
 __global__ __launch_bounds__(256) void act8_unpack_kernel(
         const signed char* codes, const float* scales, I rows, int dim, O* out,
         long long ld) {
-    constexpr int CHUNKS = 4;
-    const I nc = (dim + 7) / 8, n = rows * nc;
-    const int ng = groups_of(dim);
-    for (I i0 = (I)blockIdx.x * 256 * CHUNKS + threadIdx.x; i0 < n;
-         i0 += (I)gridDim.x * 256 * CHUNKS) {
-        i8x8 raw[CHUNKS];
-        float scale[CHUNKS];
-        I row[CHUNKS];
-        int c[CHUNKS];
+    const I nc = (dim + 7) / 8, i = (I)blockIdx.x * 256 + threadIdx.x;
+    const I row = i / nc;
+    const int c = (int)(i - row * nc) * 8;
+    if (row >= rows) return;
+    const signed char* p = codes + (long long)row * dim;
+    i8x8 raw;
+    if (dim >= 8) {
+        raw = *reinterpret_cast<const i8x8*>(p + (c < dim - 8 ? c : dim - 8));
+    } else {
         #pragma unroll
-        for (int k = 0; k < CHUNKS; ++k) {
-            const I at = i0 + k * 256, i = at < n ? at : n - 1;
-            row[k] = i / nc;
-            c[k] = (int)(i - row[k] * nc) * 8;
-            const signed char* p = codes + (long long)row[k] * dim;
-            if (dim >= 8) {
-                raw[k] = *reinterpret_cast<const i8x8*>(
-                    p + (c[k] < dim - 8 ? c[k] : dim - 8));
-            } else {
-                #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    raw[k][j] = j < dim ? p[j] : (signed char)0;
-            }
-            scale[k] = scales[(long long)row[k] * ng + c[k] / ACT8_GROUP];
-        }
-        #pragma unroll
-        for (int k = 0; k < CHUNKS; ++k) {
-            if (i0 + k * 256 >= n) break;
-            float v[8];
-            unpack8(raw[k], c[k], dim, dim % 8 == 0, v);
-            #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] *= scale[k];
-            store8(out + (long long)row[k] * ld + c[k], dim - c[k], v);
-        }
+        for (int j = 0; j < 8; ++j) raw[j] = j < dim ? p[j] : (signed char)0;
     }
+    const float scale =
+        scales[(long long)row * groups_of(dim) + c / ACT8_GROUP];
+    float v[8];
+    unpack8(raw, c, dim, dim % 8 == 0, v);
+    #pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= scale;
+    store8(out + (long long)row * ld + c, dim - c, v);
 }

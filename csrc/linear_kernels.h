@@ -154,8 +154,7 @@ __device__ __forceinline__ void finish8(float* v, long long m, int n, int left,
     } else if (e.keep == KEEP_FULL) {
         if (on) store8((T*)e.kept + m * N + n, left, v);
     } else if (e.keep == KEEP_8BIT) {
-        const float a = max16(max8(v));
-        const Act8Scale s = act8_scale(a, a < __builtin_inff());
+        const Act8Scale s = act8_scale(max16(max8(v)));
         if (on) {
             store8_codes((signed char*)e.kept + m * N + n, left, v, s.by);
             if (n % ACT8_GROUP == 0)
@@ -178,8 +177,7 @@ __device__ __forceinline__ void finish8(float* v, long long m, int n, int left,
         #pragma unroll
         for (int i = 0; i < 8; ++i)
             v[i] = whole || i < left ? (float)(T)v[i] : 0.0f;
-        const float a = max16(max8(v));
-        const Act8Scale s = act8_scale(a, a < __builtin_inff());
+        const Act8Scale s = act8_scale(max16(max8(v)));
         if (on) {
             store8_codes(e.out8 + m * N + n, left, v, s.by);
             if (n % ACT8_GROUP == 0)
