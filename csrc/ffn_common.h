@@ -50,32 +50,35 @@ __device__ __forceinline__ void load8(const T* p, int left, float* v) {
     }
 }
 
-// 8 values from column c of a row of `dim`, as they lie in memory, for rows that
+// E values from column c of a row of `dim`, as they lie in memory, for rows that
 // may end inside a chunk: nothing branches between the load and its use, so that
-// many are on their way at once.  Where the chunk ends past the row, its last 8
-// values come instead, and unpack8() moves them; `c` may lie past the row.
+// many are on their way at once.  Where the chunk ends past the row, its last E
+// values come instead, and settle() moves them; `c` may lie past the row.
+template <typename V, int E, typename T>
+__device__ __forceinline__ V fetch(const T* row, int c, int dim) {
+    if (dim >= E)
+        return *reinterpret_cast<const V*>(row + (c < dim - E ? c : dim - E));
+    V v;
+    #pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = i < dim ? row[i] : (T)0.0f;
+    return v;
+}
 template <typename T>
 __device__ __forceinline__ typename Chunk<T>::V fetch8(const T* row, int c,
                                                        int dim) {
-    if (dim >= 8)
-        return *reinterpret_cast<const typename Chunk<T>::V*>(
-            row + (c < dim - 8 ? c : dim - 8));
-    typename Chunk<T>::V v;
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < dim ? row[i] : (T)0.0f;
-    return v;
+    return fetch<typename Chunk<T>::V, 8>(row, c, dim);
 }
 
-// What fetch8 brought, with the columns where they belong and zeros in those that
+// What fetch() brought, with the columns where they belong and zeros in those that
 // are not there: shifted down as a whole, and only where a lane's chunk ends past
 // the row (done on single values by all lanes, this took as long as the rest of
 // the norm).
-template <typename V>
-__device__ __forceinline__ V settle8(V raw, int c, int dim) {
-    constexpr int W = sizeof(V) / 4, SZ = sizeof(V) / 8;
-    const int over = dim >= 8 ? c - (dim - 8) : c;
+template <int E, typename V>
+__device__ __forceinline__ V settle(V raw, int c, int dim) {
+    constexpr int W = sizeof(V) / 4, SZ = sizeof(V) / E;
+    const int over = dim >= E ? c - (dim - E) : c;
     if (!__any(over > 0)) return raw;
-    const int by = over <= 0 ? 0 : over < 8 && dim >= 8 ? over * SZ : 8 * SZ;
+    const int by = over <= 0 ? 0 : over < E && dim >= E ? over * SZ : E * SZ;
     union { V v; unsigned d[W]; } u;
     u.v = raw;
     #pragma unroll
@@ -87,12 +90,12 @@ __device__ __forceinline__ V settle8(V raw, int c, int dim) {
                                              u.d[i], b)
                 : u.d[i];
     #pragma unroll
-    for (int b = 4; b < 8 * SZ; b *= 2)
+    for (int b = SZ < 4 ? 4 : SZ; b < E * SZ; b *= 2)
         #pragma unroll
         for (int i = 0; i < W; ++i)
             u.d[i] = by & b ? (i + b / 4 < W ? u.d[i + b / 4] : 0u) : u.d[i];
     #pragma unroll
-    for (int i = 0; i < W; ++i) u.d[i] = by == 8 * SZ ? 0u : u.d[i];
+    for (int i = 0; i < W; ++i) u.d[i] = by == E * SZ ? 0u : u.d[i];
     return u.v;
 }
 
@@ -100,7 +103,7 @@ __device__ __forceinline__ V settle8(V raw, int c, int dim) {
 template <typename V>
 __device__ __forceinline__ void unpack8(V raw, int c, int dim, bool whole,
                                         float* v) {
-    if (!whole) raw = settle8(raw, c, dim);
+    if (!whole) raw = settle<8>(raw, c, dim);
     #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = (float)raw[i];
 }

@@ -52,15 +52,10 @@ __device__ __forceinline__ void dma16(u32x4 desc, unsigned lds, int voff,
                  : "scc");
 }
 
-// every copy into LDS and every read of LDS by this wave is done, and all WAVES
-// that share the tile have come here
-template <int WAVES>
+// every copy into LDS and every read of LDS by this wave is done, and the whole
+// block has come here
 __device__ __forceinline__ void stage_wait() {
-    if (WAVES == 1)
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    else
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier"
-                     ::: "memory");
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
 __device__ __forceinline__ u32x4 buffer_desc(const void* p, long long bytes) {
@@ -258,15 +253,13 @@ struct Gemm {
                                     const Operand& b_, int M_, int N_, int K_,
                                     int m0_, int n0_)
         : a(a_), b(b_), M(M_), N(N_), K(K_), m0(m0_), n0(n0_) {
-        // a wave by itself may be one of several in its block
-        tid = NW == 1 ? threadIdx.x & 63 : threadIdx.x;
+        tid = threadIdx.x;
         lane = tid & 63;
         wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         wm = wave / WN;
         wn = wave % WN;
         base = (lds_byte*)lds;
-        base_at = __builtin_amdgcn_readfirstlane(
-            (unsigned)(unsigned long long)base);
+        base_at = (unsigned)(unsigned long long)base;
         #pragma unroll
         for (int i = 0; i < TA::COPIES; ++i)
             va[i] = TA::source(wave, lane, i, (int)a.ld);
@@ -374,7 +367,7 @@ struct Gemm {
         if (mb)
             TB::mend(base + buf * STAGE + TA::BYTES, tid, THREADS, K - k,
                      N - n0, ob, at_b(k), (int)b.ld);
-        if (ma || mb) stage_wait<NW>();
+        if (ma || mb) stage_wait();
     }
 
     // acc += a b over k0..k1; nobody uses the block's LDS
@@ -391,7 +384,7 @@ struct Gemm {
         constexpr int HALF = COPIES / 2, REST = COPIES - HALF;
         int buf = 0, k = k0;
         const bool one = k0 + BK >= k1;
-        stage_wait<NW>();
+        stage_wait();
         if (one) {
             mend(k, k1, 0);
         } else {
@@ -405,7 +398,7 @@ struct Gemm {
             step<0, true, HALF, REST>(p, 1);
             step<1, true, 0, 0>(p, 2);
             step<0, true, 0, 0>(p, 3);
-            stage_wait<NW>();
+            stage_wait();
             advance(buf);
             step<1, true, 0, HALF>(base + (buf ^ 1) * STAGE, 0);
         }
@@ -414,7 +407,7 @@ struct Gemm {
             step<0, true, HALF, REST>(p, 1);
             step<1, true, 0, 0>(p, 2);
             step<0, true, 0, 0>(p, 3);
-            stage_wait<NW>();
+            stage_wait();
             buf ^= 1;
             mend(k + BK, k1, buf);
             step<1, true, 0, 0>(base + buf * STAGE, 0);

@@ -127,16 +127,10 @@ static void product(at::ScalarType type, const Operand& a, const Operand& b,
         if (M <= THIN_ROWS && !quantises && !a.lo) {
             const dim3 grid((unsigned)((N + 31) / 32),
                             (unsigned)((M + 31) / 32));
-            // 8 waves fill a unit's LDS, 4 leave room for a second block
-            const bool wide = (long long)grid.x * grid.y <= 256;
             FFN_TYPES(type,
-                typedef Gemm<T, 32, 32, 1, 1, true, BA> G;
-                auto k = wide ? thin_kernel<T, BA, 8, EPI>
-                              : thin_kernel<T, BA, 4, EPI>;
-                const int waves = wide ? 8 : 4;
-                hipLaunchKernelGGL(k, grid, waves * 64, waves * G::LDS,
-                                   stream_now(), a, b, (int)M, (int)N,
-                                   (int)K, e));
+                auto k = thin_kernel<T, BA, EPI>;
+                hipLaunchKernelGGL(k, grid, THIN_WAVES * 64, 0, stream_now(),
+                                   a, b, (int)M, (int)N, (int)K, e));
             FFN_OK();
             *blocks = grid.y;
             return;
@@ -277,7 +271,10 @@ Mat through_act(const Mat& dy, int act, const Kept& u, const at::Tensor& bias,
     e.ld_out = p.ld;
     e.act = act;
     set_kept(e, u);
-    const int rows = finish_rows(p.rows, p.dim);
+    // all of a few rows in one block a column: their sums are the gradient of the
+    // bias at once, where a second launch costs 4 us and blocks of 16 rows win 1
+    const int rows = bias.defined() && p.rows <= 64 ? 64
+                                                    : finish_rows(p.rows, p.dim);
     Colsum sum;
     if (bias.defined()) sum.aim(e, p.rows, p.dim, bias, p.rows <= rows);
     const dim3 grid((unsigned)((p.rows + rows - 1) / rows),

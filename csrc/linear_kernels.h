@@ -216,7 +216,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(
     g.run(k0, k1);
     if (a.lo) {
         g.a.p = a.lo;
-        stage_wait<G::NW>();
+        stage_wait();
         g.run(k0, k1);
     }
 
@@ -284,25 +284,103 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(
     }
 }
 
-// Few rows: 32 x 32 results a block, k shared out among its KW waves.  Each wave
-// has stages of its own and waits for nobody before the end.  What bounds it is
-// the weight's way from memory, 8 KB a wave under way.  (Fragments straight from
-// memory, without LDS, took 17 us for 20 x 1500 by 10000: a load of 16 bytes from
-// each of 32 rows is 64 requests to the cache, a copy of 8 rows 16 at most.)
-template <typename T, bool BA, int KW, int EPI>
-__global__ __launch_bounds__(KW * 64) void thin_kernel(
+// Few rows: 32 x 32 results a block, k shared out among its 8 waves, which wait
+// for nobody before the end.  What bounds it is the weight's way from memory, so
+// each wave has two steps of 128 bytes of k on their way at once, in registers:
+// copies into LDS would need 16 KB of it a wave.  From there they go through LDS
+// (one stage a wave, no barrier: a wave's accesses keep their order) to get from
+// rows of memory to fragments.  20 x 1500 by 10000 in bf16, us: fragments
+// straight from memory 17 (16 bytes of each of 32 rows are 64 requests to the
+// cache, 128 bytes of 8 rows 16 at most), copies into two stages a wave 13, this
+// 10.6; three steps leave registers for one block a unit only, 12.8.
+#define THIN_WAVES 8
+#define THIN_AHEAD 2
+template <typename T, bool BA, int EPI>
+__global__ __launch_bounds__(THIN_WAVES * 64, 4) void thin_kernel(
         Operand a, Operand b, int M, int N, int K, EpiArgs e) {
     typedef Gemm<T, 32, 32, 1, 1, true, BA> G;
-    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
-    const int wave = threadIdx.x >> 6;
+    typedef typename G::TA TA;
+    typedef typename G::TB TB;
+    constexpr int E = TA::E, STAGE = G::STAGE > 32 * 36 * 4 ? G::STAGE
+                                                           : 32 * 36 * 4;
+    typedef T V __attribute__((ext_vector_type(E), aligned(sizeof(T))));
+    typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+    __shared__ __attribute__((aligned(1024)))
+        unsigned char lds[THIN_WAVES][STAGE];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int m0 = blockIdx.y * 32, n0 = blockIdx.x * 32;
+    lds_byte* own = (lds_byte*)lds[wave];
     const int steps = (K + G::BK - 1) / G::BK;
-    const int per = (steps + KW - 1) / KW * G::BK;
-    const int k0 = __builtin_amdgcn_readfirstlane(wave * per);
-    const int k1 = K - k0 < per ? K : k0 + per;
-    unsigned char* own = lds + wave * G::LDS;
-    G g(own, a, b, M, N, K, m0, n0);
-    if (k0 < k1) g.run(k0, k1);
+    const int per = (steps + THIN_WAVES - 1) / THIN_WAVES;
+    const int s0 = wave * per, s1 = s0 + per < steps ? s0 + per : steps;
+    f32x16 acc;
+    #pragma unroll
+    for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
+    V x[THIN_AHEAD][4], y[THIN_AHEAD][4];
+    // this lane's chunk i: stored row and first value in it
+    auto row_a = [&](int i) { return i * TA::RPC + lane / TA::CH; };
+    auto row_b = [&](int i) { return i * TB::RPC + lane / TB::CH; };
+    auto col_a = [&](int i) {
+        return ((lane % TA::CH) ^ TA::swizzle(row_a(i))) * E;
+    };
+    auto col_b = [&](int i) {
+        return ((lane % TB::CH) ^ TB::swizzle(row_b(i))) * E;
+    };
+    auto load = [&](int s, V* to_x, V* to_y) {
+        if (s >= s1) return;
+        const int k = s * G::BK;
+        // rows that are not there: the last one's values, for results that are
+        // not written
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int m = m0 + row_a(i);
+            to_x[i] = fetch<V, E>(
+                (const T*)a.p + (long long)(m < M ? m : M - 1) * a.ld,
+                k + col_a(i), K);
+            const int r = (BA ? n0 : k) + row_b(i), end = BA ? N : K;
+            to_y[i] = fetch<V, E>(
+                (const T*)b.p + (long long)(r < end ? r : end - 1) * b.ld,
+                (BA ? k : n0) + col_b(i), BA ? K : N);
+        }
+    };
+    const int at_a = TA::lane_at(lane, 0), at_b = TB::lane_at(lane, 0);
+    auto use = [&](int s, const V* from_x, const V* from_y) {
+        if (s >= s1) return;
+        const int k = s * G::BK;
+        const bool last = k + G::BK > K;
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            V p = from_x[i], q = from_y[i];
+            if (last) {
+                p = settle<E>(p, k + col_a(i), K);
+                if constexpr (BA) {
+                    q = settle<E>(q, k + col_b(i), K);
+                } else if (k + row_b(i) >= K) {
+                    #pragma unroll
+                    for (int j = 0; j < E; ++j) q[j] = (T)0.0f;
+                }
+            }
+            if constexpr (!BA)
+                if (n0 + 32 > N) q = settle<E>(q, n0 + col_b(i), N);
+            *(lds_u32x4*)(own + i * 1024 + lane * 16) =
+                __builtin_bit_cast(u32x4, p);
+            *(lds_u32x4*)(own + TA::BYTES + i * 1024 + lane * 16) =
+                __builtin_bit_cast(u32x4, q);
+        }
+        #pragma unroll
+        for (int j = 0; j < 4; ++j)
+            acc = Mfma<T>::go(TB::frag(own + TA::BYTES, at_b, j),
+                              TA::frag(own, at_a, j), acc);
+    };
+    #pragma unroll
+    for (int d = 0; d < THIN_AHEAD; ++d) load(s0 + d, x[d], y[d]);
+    for (int s = s0; s < s1; s += THIN_AHEAD) {
+        #pragma unroll
+        for (int d = 0; d < THIN_AHEAD; ++d) {
+            use(s + d, x[d], y[d]);
+            load(s + d + THIN_AHEAD, x[d], y[d]);
+        }
+    }
     const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 8;
     const bool whole = n0 + 32 <= N;
     Extra<T> extra;
@@ -311,14 +389,23 @@ __global__ __launch_bounds__(KW * 64) void thin_kernel(
         fetch_extra<T, EPI>(extra, e, m0 + r < M ? m0 + r : M - 1, n0 + c, N);
         if (EPI == EPI_FORWARD) load_bias<T>(e, n0 + c, N, bias);
     }
-    g.stage_out(own, 0);
+    constexpr int LD = 36;
+    float* out = reinterpret_cast<float*>(lds[wave]) + (lane & 31) * LD +
+                 4 * (lane >> 5);
+    #pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        f32x4 v;
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = acc[4 * g + i];
+        *reinterpret_cast<f32x4*>(out + 8 * g) = v;
+    }
     __syncthreads();
     if (threadIdx.x < 128) {
         float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         #pragma unroll
-        for (int w = 0; w < KW; ++w) {
-            const float* p = reinterpret_cast<const float*>(
-                lds + w * G::LDS) + r * G::OUT_LD + c;
+        for (int w = 0; w < THIN_WAVES; ++w) {
+            const float* p = reinterpret_cast<const float*>(lds[w]) + r * LD +
+                             c;
             #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] += p[i];
         }
@@ -326,7 +413,7 @@ __global__ __launch_bounds__(KW * 64) void thin_kernel(
                         whole, e, bias, extra, sums);
     }
     if (EPI == EPI_GRAD && e.colsum) {
-        float* all = reinterpret_cast<float*>(lds);
+        float* all = reinterpret_cast<float*>(lds[0]);
         __syncthreads();
         if (threadIdx.x < 128) {
             #pragma unroll
