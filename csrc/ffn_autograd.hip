@@ -2,6 +2,7 @@
 // is kept for the backward pass, and the backward pass itself.
 #include "ffn_ops.h"
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 
 namespace ffn {
@@ -67,6 +68,27 @@ static bool recording(std::initializer_list<Tensor> all) {
     if (!at::GradMode::is_enabled()) return false;
     for (const Tensor& t : all) if (wants_grad(t)) return true;
     return false;
+}
+
+// A leaf's gradient goes to it on the stream on which its first graph that still
+// lives was recorded.  Captured, that would be work on a stream that is not part
+// of the capture, which the autograd engine's thread does not survive.
+static void check_capture(std::initializer_list<Tensor> all) {
+    const auto stream = c10::hip::getCurrentHIPStream();
+    hipStreamCaptureStatus status;
+    if (hipStreamIsCapturing(stream, &status) == hipSuccess &&
+        status == hipStreamCaptureStatusNone)
+        return;
+    for (const Tensor& t : all) {
+        if (!wants_grad(t) || !t.is_leaf()) continue;
+        const auto sink = torch::autograd::impl::try_get_grad_accumulator(t);
+        if (!sink) continue;
+        const auto theirs = sink->stream();
+        TORCH_CHECK(!theirs.has_value() || theirs->id() == stream.id(),
+                    "a graph recorded on another stream keeps a parameter or "
+                    "input of this captured call: free that graph (its outputs)"
+                    " before the capture begins");
+    }
 }
 
 static void check_once(const char* name) {
@@ -139,8 +161,10 @@ Tensor layer_norm(Tensor x, c10::optional<Tensor> weight,
     check_values(x, "x");
     check_norm_params(x, gamma, beta, "weight", "bias");
     const at::DeviceGuard guard(x.device());
-    if (recording({x, gamma, beta}))
+    if (recording({x, gamma, beta})) {
+        check_capture({x, gamma, beta});
         return NormFn::apply(x, maybe(gamma), maybe(beta), eps, act8);
+    }
     return norm_forward(as_rows(x), contiguous_or_none(gamma),
                         contiguous_or_none(beta), eps, false, false, false,
                         false).y.t.view(x.sizes());
@@ -222,8 +246,10 @@ Tensor linear_act(Tensor x, Tensor weight, c10::optional<Tensor> bias,
                     r.sizes());
     }
     const at::DeviceGuard guard(x.device());
-    if (recording({x, weight, b, r}))
+    if (recording({x, weight, b, r})) {
+        check_capture({x, weight, b, r});
         return LinearFn::apply(x, weight, maybe(b), maybe(r), act, act8);
+    }
     Mat rm;
     if (r.defined()) rm = as_rows(r);
     return linear_forward(as_rows(x), as_rows(weight), contiguous_or_none(b),
@@ -326,9 +352,11 @@ Tensor ffn_block(Tensor x, c10::optional<Tensor> norm_weight,
     check_params(x, c2, x.size(-1), "b2");
     check_act(act);
     const at::DeviceGuard guard(x.device());
-    if (recording({x, gamma, beta, w1, c1, w2, c2}))
+    if (recording({x, gamma, beta, w1, c1, w2, c2})) {
+        check_capture({x, gamma, beta, w1, c1, w2, c2});
         return BlockFn::apply(x, maybe(gamma), maybe(beta), w1, maybe(c1), w2,
                               maybe(c2), act, eps, act8);
+    }
     const Mat m = as_rows(x);
     const NormOut n = norm_forward(m, contiguous_or_none(gamma),
                                    contiguous_or_none(beta), eps, false, false,

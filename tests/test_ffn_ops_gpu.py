@@ -547,6 +547,35 @@ def test_captured_steps():
                 assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("which", ["norm", "linear", "block"])
+def test_capture_refuses_a_living_graph_of_its_leaves(which):
+    args = block_args(40, 24, 56, BF)
+    x, gamma, beta, w1, b1 = args[:5]
+    call = {"norm": lambda: gt.layer_norm(x, gamma, beta),
+            "linear": lambda: gt.linear_act(x, w1, b1, act="gelu"),
+            "block": lambda: gt.ffn_block(*args)}[which]
+    leaves = {"norm": (x, gamma, beta), "linear": (x, w1, b1),
+              "block": args}[which]
+    dy = torch.ones_like(call())
+    want = torch.autograd.grad(call(), leaves, dy)
+    living = call()
+    graph = torch.cuda.CUDAGraph()
+    mark = torch.zeros(1, device=DEV)
+    with pytest.raises(RuntimeError, match="free that graph"):
+        with torch.cuda.graph(graph):
+            mark += 1
+            call()
+    del living, graph
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(call(), leaves, dy)
+        twice = call()          # a second call of one capture is not refused
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_autocast_keeps_fp32_parameters():
     block = gt.FFNBlock(96, 192, act8=True).to(DEV)
     x = make(50, 96)
