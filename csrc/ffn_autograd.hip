@@ -23,8 +23,9 @@ static void check_values(const Tensor& x, const char* name) {
                 x.scalar_type());
     TORCH_CHECK(x.dim() >= 1, name, " must have at least one dimension");
     TORCH_CHECK(x.size(-1) > 0, name, "'s last dimension must not be empty");
+    // a launch has less than 2^32 threads, and a thread at least four rows
     TORCH_CHECK(x.size(-1) < (1LL << 30) &&
-                x.numel() / x.size(-1) < (1LL << 30), name, " of shape ",
+                x.numel() / x.size(-1) <= 1000000000, name, " of shape ",
                 x.sizes(), " is too large");
 }
 
@@ -160,6 +161,8 @@ Tensor layer_norm(Tensor x, c10::optional<Tensor> weight,
     const Tensor gamma = or_none(weight), beta = or_none(bias);
     check_values(x, "x");
     check_norm_params(x, gamma, beta, "weight", "bias");
+    TORCH_CHECK(x.size(-1) < (1LL << 25), "rows of ", x.size(-1),
+                " are too long");
     const at::DeviceGuard guard(x.device());
     if (recording({x, gamma, beta})) {
         check_capture({x, gamma, beta});

@@ -262,10 +262,12 @@ template <bool FAST>
 __device__ __forceinline__ float act_value(float u, int act) {
     if (act == ACT_RELU) return u > 0.0f || u != u ? u : 0.0f;
     if (act == ACT_GELU) {
-        // u Phi(u): u - u q above 0, u q below
+        // u Phi(u): u - u q above 0, u q below; q = 0 from 16 on, and infinity
+        // times 0 is not 0
         float e;
         const float q = normal_tail<FAST>(u, &e);
-        return __builtin_fmaf(-fabsf(u), q, u > 0.0f || u != u ? u : 0.0f);
+        return __builtin_fmaf(-fminf(fabsf(u), 16.0f), q,
+                              u > 0.0f || u != u ? u : 0.0f);
     }
     if (act == ACT_SILU) {
         if (FAST) return u * __builtin_amdgcn_rcpf(
@@ -278,18 +280,20 @@ __device__ __forceinline__ float act_value(float u, int act) {
 template <bool FAST>
 __device__ __forceinline__ float act_slope(float u, int act) {
     if (act == ACT_GELU) {
-        // Phi(u) + u phi(u), phi(u) = e / sqrt(2 pi)
+        // Phi(u) + u phi(u), phi(u) = e / sqrt(2 pi); a NaN is in cdf
         float e;
         const float q = normal_tail<FAST>(u, &e);
         const float cdf = 0.5f + __builtin_copysignf(0.5f - q, u);
-        return __builtin_fmaf(u * e, 0.3989422804014327f, cdf);
+        return __builtin_fmaf(__builtin_amdgcn_fmed3f(u, -16.0f, 16.0f) * e,
+                              0.3989422804014327f, cdf);
     }
     if (act == ACT_SILU) {
         const float s = FAST
             ? __builtin_amdgcn_rcpf(
                   1.0f + __builtin_amdgcn_exp2f(u * -1.44269504089f))
             : 1.0f / (1.0f + expf(-u));
-        return s * __builtin_fmaf(u, 1.0f - s, 1.0f);
+        return s * __builtin_fmaf(__builtin_amdgcn_fmed3f(u, -128.0f, 128.0f),
+                                  1.0f - s, 1.0f);
     }
     return 1.0f;
 }

@@ -105,9 +105,7 @@ Mat unpack(const at::Tensor& codes, const at::Tensor& scales,
     }
     const long long n = rows * ((dim + 7) / 8);
     if (!n) return out;
-    TORCH_CHECK(n < (1LL << 38), "8-bit form of ", rows, " x ", dim,
-                " is too large");
-    const unsigned grid = (unsigned)((n + 255) / 256);
+    const int grid = (int)std::min<long long>((n + 255) / 256, 1 << 22);
     FFN_TYPES(type, FFN_COUNT(n,
         auto k = act8_unpack_kernel<T, I>;
         hipLaunchKernelGGL(k, grid, 256, 0, stream_now(),

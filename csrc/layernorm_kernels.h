@@ -520,23 +520,26 @@ template <typename O, typename I>
 __global__ __launch_bounds__(256) void act8_unpack_kernel(
         const signed char* codes, const float* scales, I rows, int dim, O* out,
         long long ld) {
-    const I nc = (dim + 7) / 8, i = (I)blockIdx.x * 256 + threadIdx.x;
-    const I row = i / nc;
-    const int c = (int)(i - row * nc) * 8;
-    if (row >= rows) return;
-    const signed char* p = codes + (long long)row * dim;
-    i8x8 raw;
-    if (dim >= 8) {
-        raw = *reinterpret_cast<const i8x8*>(p + (c < dim - 8 ? c : dim - 8));
-    } else {
+    const I nc = (dim + 7) / 8;
+    // once, but for more chunks than a launch may have threads
+    for (I i = (I)blockIdx.x * 256 + threadIdx.x; i < rows * nc;
+         i += (I)gridDim.x * 256) {
+        const I row = i / nc;
+        const int c = (int)(i - row * nc) * 8;
+        const signed char* p = codes + (long long)row * dim;
+        i8x8 raw;
+        if (dim >= 8) {
+            raw = *reinterpret_cast<const i8x8*>(p + (c < dim - 8 ? c : dim - 8));
+        } else {
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) raw[j] = j < dim ? p[j] : (signed char)0;
+        }
+        const float scale =
+            scales[(long long)row * groups_of(dim) + c / ACT8_GROUP];
+        float v[8];
+        unpack8(raw, c, dim, dim % 8 == 0, v);
         #pragma unroll
-        for (int j = 0; j < 8; ++j) raw[j] = j < dim ? p[j] : (signed char)0;
+        for (int j = 0; j < 8; ++j) v[j] *= scale;
+        store8(out + (long long)row * ld + c, dim - c, v);
     }
-    const float scale =
-        scales[(long long)row * groups_of(dim) + c / ACT8_GROUP];
-    float v[8];
-    unpack8(raw, c, dim, dim % 8 == 0, v);
-    #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= scale;
-    store8(out + (long long)row * ld + c, dim - c, v);
 }

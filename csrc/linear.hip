@@ -87,7 +87,7 @@ static void launch(const Operand& a, const Operand& b, int M, int N, int K,
     typedef Gemm<T, BM, BN, WM, WN, AA, BA> G;
     const auto s = stream_now();
     const long long tm = (M + BM - 1) / BM, tn = (N + BN - 1) / BN;
-    TORCH_CHECK(tm * tn < (1LL << 31), "product of ", M, " x ", N,
+    TORCH_CHECK(tm * tn < (1LL << 32) / G::THREADS, "product of ", M, " x ", N,
                 " is too large");
     const int steps = (K + G::BK - 1) / G::BK;
     const int per = (steps + splits - 1) / splits;

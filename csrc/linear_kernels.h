@@ -9,7 +9,7 @@ enum Epilogue { EPI_FORWARD = 0, EPI_GRAD = 1, EPI_PLAIN = 2 };
 enum Keep { KEEP_NONE = 0, KEEP_FULL = 1, KEEP_BITS = 2, KEEP_8BIT = 3 };
 
 struct EpiArgs {
-    void* out;             // [M, N] of T (EPI_PLAIN: of float where out_f32)
+    void* out;             // [M, N] of T
     long long ld_out;
     void* out_lo;          // EPI_GRAD: what rounding to `out` left, or null
     const void* bias;      // [N] of T (of float where bias_f32) or null
@@ -22,7 +22,7 @@ struct EpiArgs {
     // EPI_GRAD: sums of `out` over the rows, or null: [row blocks, N] of float,
     // or, where all rows are one block's, [N] of float or of T
     void* colsum;
-    int act, keep, bias_f32, out_f32, colsum_out;
+    int act, keep, bias_f32, colsum_out;
 };
 enum ColsumOut { COLSUM_FLOAT = 0, COLSUM_T = 1 };
 
@@ -99,9 +99,7 @@ __device__ __forceinline__ void finish8(float* v, long long m, int n, int left,
     constexpr bool FAST = IsHalf<T>::value;
     const bool on = left > 0;
     if (EPI == EPI_PLAIN) {
-        if (!on) return;
-        if (e.out_f32) store8((float*)e.out + m * e.ld_out + n, left, v);
-        else store8((T*)e.out + m * e.ld_out + n, left, v);
+        if (on) store8((T*)e.out + m * e.ld_out + n, left, v);
         return;
     }
     if (EPI == EPI_GRAD) {

@@ -272,6 +272,32 @@ def test_linear_bad_values_stay_in_their_row(m, k):
         assert rows == [m // 2]
 
 
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("t", [BF, HF, FP])
+@pytest.mark.parametrize("m", [5, 70])
+def test_linear_infinite_values(act, t, m):
+    """Where u is infinite, every activation of it is, and its slope is 1; it
+    is NaN where u is."""
+    k, n = 40, 24
+    x = make(m, k, t=t)
+    w = make(n, k, t=t, seed=1)
+    with torch.no_grad():
+        x[1, 3] = float("inf")
+        x[3, 3] = float("nan")
+        w[:, 3] = w[:, 3].abs() + 0.125
+    dy = make(m, n, t=t, seed=2, grad=False)
+    y = gt.linear_act(x, w, act=act)
+    assert bool((y[1] == float("inf")).all())
+    assert bool(torch.isnan(y[3]).all())
+    dx, = torch.autograd.grad(y, x, dy)
+    straight, = torch.autograd.grad(gt.linear_act(x, w), x, dy)
+    assert torch.equal(dx[1], straight[1])
+    if act in ("gelu", "silu"):
+        assert bool(torch.isnan(dx[3]).all())
+    others = [i for i in range(m) if i not in (1, 3)]
+    assert bool(torch.isfinite(y[others]).all() & torch.isfinite(dx[others]).all())
+
+
 def test_linear_keeps_results_without_gradients():
     x, w = make(33, 77, t=BF), make(50, 77, t=BF, seed=1)
     y = gt.linear_act(x, w, act="gelu")
@@ -333,6 +359,20 @@ def test_act8_edges_are_the_cpu_ones():
     p, q = gt.act8_pack(x.to(DEV)), gt.act8_pack(x)
     assert torch.equal(p.codes.cpu(), q.codes)
     assert torch.equal(p.scales.cpu().nan_to_num(-1), q.scales.nan_to_num(-1))
+
+
+def test_act8_more_chunks_than_threads():
+    """9 rows of 2^30 - 8 values: more chunks of 8 than one launch has threads
+    for, the last of them against the codes."""
+    rows, dim = 9, 2 ** 30 - 8
+    codes = torch.zeros(rows, dim, dtype=torch.int8, device=DEV)
+    codes[-1, -1000:] = torch.arange(1000, device=DEV).sub(500).clamp(-127, 127)
+    codes[0, :3] = 7
+    scales = torch.full((rows, -(-dim // 128)), 0.5, device=DEV)
+    x = gt.act8_unpack(codes, scales, BF)
+    assert torch.equal(x[-1, -1000:], codes[-1, -1000:].to(BF) * 0.5)
+    assert torch.equal(x[0, :8], codes[0, :8].to(BF) * 0.5)
+    assert not bool(x[-2].any())
 
 
 def test_act8_strides():
@@ -626,6 +666,15 @@ def test_refusals_gpu():
     with pytest.raises(RuntimeError, match="act8_unpack gives"):
         gt.act8_unpack(torch.zeros(3, 8, dtype=torch.int8, device=DEV),
                        torch.zeros(3, 1, device=DEV), torch.float64)
+    one = torch.zeros(1, 1, device=DEV)     # views of it hold no memory
+    with pytest.raises(RuntimeError, match="too large"):
+        gt.act8_pack(one.expand(2 ** 30, 1))
+    with pytest.raises(RuntimeError, match="too large"):
+        gt.linear_act(one.expand(2 ** 30, 1), one)
+    with pytest.raises(RuntimeError, match="too large"):
+        gt.linear_act(one.expand(1, 4000001), one.expand(1, 4000001))
+    with pytest.raises(RuntimeError, match="too long"):
+        gt.layer_norm(one.expand(1, 2 ** 25))
     for f in (lambda: gt.layer_norm(x), lambda: gt.linear_act(x, w)):
         with pytest.raises(RuntimeError, match="second derivative"):
             torch.autograd.grad(f().sum(), x, create_graph=True)
