@@ -218,12 +218,16 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
             // the weight's gradient is rounded once; x unpacked from 8 bits
             // rounds once more, and p would be the third
             const bool act8 = need_w && s[2].defined();
-            Mat p = through_act(as_rows(dy), act, u, need_b ? s[6] : Tensor(),
-                                &db, act8);
+            // without an activation the bias's gradient comes with dW, or alone
+            const bool plain = need_b && act == 0;
+            Mat p = through_act(as_rows(dy), act, u,
+                                need_b && !plain ? s[6] : Tensor(), &db, act8);
             if (need_w)
                 dw = weight_grad(p, act8
                     ? unpack(s[2], s[3], dy.scalar_type(), true)
-                    : as_rows(s[0]));
+                    : as_rows(s[0]), plain ? s[6] : Tensor(), &db);
+            else if (plain)
+                db = row_sums(p, s[6].scalar_type());
             p.lo = Tensor();
             if (need_x)
                 dx = input_grad(p, as_rows(s[1]), 0, Kept(), Tensor(), nullptr,
@@ -307,8 +311,10 @@ struct BlockFn : public torch::autograd::Function<BlockFn> {
         };
         Tensor dx, dw1, db1, dw2, db2;
         NormGrads g;
-        if (need(5)) dw2 = weight_grad(d, kept(2, 7));
-        if (need(6)) db2 = row_sums(d, b2.scalar_type());
+        if (need(5))
+            dw2 = weight_grad(d, kept(2, 7), need(6) ? b2 : Tensor(), &db2);
+        else if (need(6))
+            db2 = row_sums(d, b2.scalar_type());
         const bool norm = need(0) || need(1) || need(2);
         const bool bias = need(4);
         if (norm || need(3) || bias) {
@@ -331,7 +337,8 @@ struct BlockFn : public torch::autograd::Function<BlockFn> {
                 if (need(0)) dx = g.dx.view(dy.sizes());
             }
             if (!act8) p.lo = Tensor();
-            if (need(3)) dw1 = weight_grad(p, kept(1, 5));
+            if (need(3))
+                dw1 = weight_grad(p, kept(1, 5), Tensor(), nullptr);
         }
         return {dx, g.dgamma, g.dbeta, dw1, db1, dw2, db2, Tensor(), Tensor(),
                 Tensor()};

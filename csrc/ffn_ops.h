@@ -49,14 +49,17 @@ struct LinearOut { Mat y; Kept u; Packed y8; };
 LinearOut linear_forward(const Mat& x, const Mat& w, const at::Tensor& bias,
                          const Mat* res, int act, bool keep, bool act8,
                          bool keep_y8, bool lines);
-// p = dy act'(u), and the sum of its rows in bias's type where bias is defined.
-// `split`: p keeps what rounding leaves, where the activation makes it round.
+// p = dy act'(u), and the sum of its rows in bias's type where bias is defined
+// (without an activation: dy, and no sum).  `split`: p keeps what rounding
+// leaves, where the activation makes it round.
 Mat through_act(const Mat& dy, int act, const Kept& u, const at::Tensor& bias,
                 at::Tensor* dbias, bool split);
 // dx = p W, rounded, then through the activation below as through_act does
 Mat input_grad(const Mat& p, const Mat& w, int act, const Kept& u,
                const at::Tensor& bias, at::Tensor* dbias, bool split);
-at::Tensor weight_grad(const Mat& p, const Mat& x);
+// dW = p^T x, and the sum of p's rows in bias's type where bias is defined
+at::Tensor weight_grad(const Mat& p, const Mat& x, const at::Tensor& bias,
+                       at::Tensor* dbias);
 at::Tensor row_sums(const Mat& p, at::ScalarType type);
 
 // autograd entry points, bound in gtopk_ext.hip

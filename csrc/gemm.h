@@ -248,10 +248,14 @@ struct Gemm {
     int ka, kb;
     typename Mfma<T>::V xa[2][TM], xb[2][TN];
     f32x16 acc[TM][TN];
+    // Both operands across k: B may go on with a column of ones behind its N,
+    // where the last tile has room, so that C's column N is the sum of A over k.
+    static constexpr bool ONES = !AA && !BA;
+    bool one[TN], any_one;     // this lane's column of B is the one of ones
 
     __device__ __forceinline__ Gemm(unsigned char* lds, const Operand& a_,
                                     const Operand& b_, int M_, int N_, int K_,
-                                    int m0_, int n0_)
+                                    int m0_, int n0_, bool ones)
         : a(a_), b(b_), M(M_), N(N_), K(K_), m0(m0_), n0(n0_) {
         tid = threadIdx.x;
         lane = tid & 63;
@@ -272,6 +276,12 @@ struct Gemm {
         #pragma unroll
         for (int j = 0; j < TN; ++j)
             fb[j] = TB::lane_at(lane, (wn * TN + j) * 32);
+        #pragma unroll
+        for (int j = 0; j < TN; ++j)
+            one[j] = ONES && ones &&
+                     n0 + (wn * TN + j) * 32 + (lane & 31) == N;
+        any_one = ONES && ones && N >= n0 + wn * TN * 32 &&
+                  N < n0 + (wn + 1) * TN * 32;
         #pragma unroll
         for (int i = 0; i < TM; ++i)
             #pragma unroll
@@ -335,6 +345,15 @@ struct Gemm {
     template <int I, int CUR, bool LOAD, int FROM, int COUNT>
     __device__ __forceinline__ void step_rows(lds_byte* next, int ns) {
         if constexpr (I < TM) {
+            if (ONES && I == 0 && any_one) {
+                // by waves that have the column only: its 4 instructions for
+                // each fragment cost a tenth of the product
+                #pragma unroll
+                for (int j = 0; j < TN; ++j)
+                    #pragma unroll
+                    for (int e = 0; e < 16 / SZ; ++e)
+                        xb[CUR][j][e] = one[j] ? (T)1.0f : xb[CUR][j][e];
+            }
             if (LOAD) {
                 #pragma unroll
                 for (int l = I * LOADS / TM; l < (I + 1) * LOADS / TM; ++l)

@@ -92,7 +92,10 @@ static void launch(const Operand& a, const Operand& b, int M, int N, int K,
     const int steps = (K + G::BK - 1) / G::BK;
     const int per = (steps + splits - 1) / splits;
     const int parts = (steps + per - 1) / per;
-    const long long ld_part = (N + 3) / 4 * 4;
+    // the column of ones has to find room in the last tile
+    if (EPI == EPI_PLAIN && N % BN == 0) e.colsum = nullptr;
+    const int wide = EPI == EPI_PLAIN && e.colsum ? N + 1 : N;
+    const long long ld_part = (wide + 3) / 4 * 4;
     at::Tensor part;
     if (parts > 1)
         part = at::empty({parts, M, ld_part},
@@ -107,16 +110,18 @@ static void launch(const Operand& a, const Operand& b, int M, int N, int K,
     if (parts > 1) {
         const int rows = finish_rows(M, N);
         const dim3 fgrid((unsigned)((M + rows - 1) / rows),
-                         (unsigned)((N + 127) / 128));
+                         (unsigned)((wide + 127) / 128));
         auto f = finish_kernel<T, EPI, float>;
         hipLaunchKernelGGL(f, fgrid, 256, 0, s, pp, ld_part, parts, rows, M, N,
                            e);
         FFN_OK();
         *blocks = fgrid.x;
     }
+    if (EPI == EPI_PLAIN) *blocks = e.colsum ? 1 : 0;
 }
 
-// C = A B with the epilogue; `blocks`: rows of e.colsum that were written
+// C = A B with the epilogue; `blocks`: rows of e.colsum that were written (none
+// where EPI_PLAIN's sums found no room)
 template <bool AA, bool BA, int EPI>
 static void product(at::ScalarType type, const Operand& a, const Operand& b,
                     long long M, long long N, long long K, EpiArgs e,
@@ -256,10 +261,7 @@ static Mat empty_grad(long long rows, long long dim, const at::Tensor& like,
 
 Mat through_act(const Mat& dy, int act, const Kept& u, const at::Tensor& bias,
                 at::Tensor* dbias, bool split) {
-    if (act == ACT_NONE) {
-        if (bias.defined()) *dbias = row_sums(dy, bias.scalar_type());
-        return dy;
-    }
+    if (act == ACT_NONE) return dy;
     Mat p = empty_grad(dy.rows, dy.dim, dy.t, split, u);
     if (!p.rows) {
         if (bias.defined()) *dbias = at::zeros_like(bias);
@@ -318,15 +320,28 @@ Mat input_grad(const Mat& p, const Mat& w, int act, const Kept& u,
     return out;
 }
 
-at::Tensor weight_grad(const Mat& p, const Mat& x) {
+// The sum of p's rows is a column of ones on x, where the last tile has room for
+// it: by itself it reads p once more, at 17920 x 10000 in bf16 97 of 1780 us.
+at::Tensor weight_grad(const Mat& p, const Mat& x, const at::Tensor& bias,
+                       at::Tensor* dbias) {
     auto out = at::empty({p.dim, x.dim}, p.t.options());
-    if (!p.rows) return out.zero_();
+    if (bias.defined()) *dbias = at::empty({p.dim}, bias.options());
+    if (!p.rows) {
+        if (bias.defined()) dbias->zero_();
+        return out.zero_();
+    }
     EpiArgs e{};
     e.out = out.data_ptr();
     e.ld_out = x.dim;
+    if (bias.defined()) {
+        e.colsum = dbias->data_ptr();
+        e.colsum_out = bias.scalar_type() == at::kFloat ? COLSUM_FLOAT
+                                                        : COLSUM_T;
+    }
     long long blocks;
     product<false, false, EPI_PLAIN>(p.t.scalar_type(), operand(p), operand(x),
                                      p.dim, x.dim, p.rows, e, p.t, &blocks);
+    if (bias.defined() && !blocks) *dbias = row_sums(p, bias.scalar_type());
     return out;
 }
 

@@ -20,7 +20,8 @@ struct EpiArgs {
     signed char* out8;     // 8-bit form of `out`, or null
     float* out8_scale;
     // EPI_GRAD: sums of `out` over the rows, or null: [row blocks, N] of float,
-    // or, where all rows are one block's, [N] of float or of T
+    // or, where all rows are one block's, [N] of float or of T.  EPI_PLAIN: sums
+    // of A over k, [M] of float or of T, or null.
     void* colsum;
     int act, keep, bias_f32, colsum_out;
 };
@@ -193,6 +194,15 @@ __device__ __forceinline__ void put_colsum(const EpiArgs& e, long long block,
     else ((float*)e.colsum)[block * N + n] = t;
 }
 
+// the sum of A over k, which is column N of the product: `left` columns on
+template <typename T>
+__device__ __forceinline__ void put_sum(const EpiArgs& e, long long m, int left,
+                                        const float* v) {
+    #pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i == left) put_colsum<T>(e, 0, (int)m, 0, v[i]);
+}
+
 // One block, one tile of C; blockIdx.y is the part of k.  With `part` the
 // tile's fp32 sums go to part[blockIdx.y][m][n] (rows of ld_part values), and
 // finish_kernel joins them; otherwise the epilogue follows at once.
@@ -210,7 +220,8 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(
     const int k0 = blockIdx.y * kper;
     const int k1 = K - k0 < kper ? K : k0 + kper;
 
-    G g(lds, a, b, M, N, K, m0, n0);
+    const int ones = EPI == EPI_PLAIN && e.colsum ? 1 : 0;
+    G g(lds, a, b, M, N, K, m0, n0, ones);
     g.run(k0, k1);
     if (a.lo) {
         g.a.p = a.lo;
@@ -259,10 +270,11 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(
             const int m = row_of(i, q);
             const int here = m < M ? left : 0;
             if (part) {
-                if (here > 0)
+                if (m < M && left + ones > 0)
                     store8(part + ((long long)blockIdx.y * M + m) * ld_part +
-                           n, here, v);
+                           n, left + ones, v);
             } else {
+                if (ones && m < M) put_sum<T>(e, m, left, v);
                 finish8<T, EPI>(v, m, n, here, N, whole, e, bias, x[q], sums);
                 if (i + 1 < G::TM) fetch(i + 1, q);
             }
@@ -440,6 +452,7 @@ __global__ __launch_bounds__(256) void finish_kernel(
     const bool whole = (int)(blockIdx.y + 1) * 128 <= N;
     float sums[8] = {0, 0, 0, 0, 0, 0, 0, 0}, bias[8];
     if (EPI == EPI_FORWARD) load_bias<T>(e, n, N, bias);
+    const int ones = EPI == EPI_PLAIN && e.colsum ? 1 : 0;
     for (int r = r0; r < rows; r += 16) {
         const long long m = (long long)blockIdx.x * rows + r;
         const long long there = m < M ? m : M - 1;
@@ -452,11 +465,12 @@ __global__ __launch_bounds__(256) void finish_kernel(
         #pragma unroll 4
         for (int s = 0; s < splits; ++s) {
             float w[8];
-            unpack8(fetch8(part + ((long long)s * M + there) * ld_part, n, N),
-                    n, N, whole, w);
+            unpack8(fetch8(part + ((long long)s * M + there) * ld_part, n,
+                           N + ones), n, N + ones, whole, w);
             #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] += w[j];
         }
+        if (ones && m < M) put_sum<T>(e, m, left, v);
         finish8<T, EPI>(v, m, n, here, N, whole, e, bias, x, sums);
     }
     if (EPI == EPI_GRAD && e.colsum) {

@@ -185,6 +185,15 @@ def test_linear_bias(bias):
     linear_case(50, 70, 90, BF, act="gelu", bias=bias)
 
 
+@pytest.mark.parametrize("k", [1, 7, 63, 64, 128, 220, 255, 256, 300])
+@pytest.mark.parametrize("m,n", [(1, 9), (70, 260), (2500, 40)])
+@pytest.mark.parametrize("t,bias", [(BF, "t"), (HF, "fp32"), (FP, "t")])
+def test_linear_bias_gradient_beside_the_weights(k, m, n, t, bias):
+    """The last tile of dW has room for the sum of the rows, or has none; the
+    sum over many rows goes in parts or in one."""
+    linear_case(m, k, n, t, bias=bias)
+
+
 @pytest.mark.parametrize("m,k,n", [(2500, 300, 40), (40, 3100, 70),
                                    (70, 50, 2500), (2100, 520, 530)])
 @pytest.mark.parametrize("t", [BF, FP])
