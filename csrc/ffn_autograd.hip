@@ -120,6 +120,11 @@ static Maybe maybe(const Tensor& t) {
     return t.defined() ? Maybe(t) : Maybe();
 }
 
+// a view costs the host as much as an allocation: none where the shape is right
+static Tensor shaped(const Tensor& t, at::IntArrayRef sizes) {
+    return t.sizes() == sizes ? t : t.view(sizes);
+}
+
 static Tensor contiguous_or_none(const Tensor& t) {
     return t.defined() ? t.contiguous() : t;
 }
@@ -134,10 +139,10 @@ struct NormFn : public torch::autograd::Function<NormFn> {
         NormOut o = norm_forward(m, contiguous_or_none(gamma),
                                  contiguous_or_none(beta), eps, true, act8,
                                  false, false);
-        ctx->save_for_backward({act8 ? Tensor() : x, gamma, beta, o.mean,
-                                o.rstd, o.x8.codes, o.x8.scales});
+        ctx->save_for_backward({act8 ? Tensor() : x, gamma, beta, o.stats,
+                                o.x8.codes, o.x8.scales});
         ctx->saved_data["inputs"] = present({x, gamma, beta});
-        return o.y.t.view(x.sizes());
+        return shaped(o.y.t, x.sizes());
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -148,10 +153,10 @@ struct NormFn : public torch::autograd::Function<NormFn> {
         const Mat d = as_rows(dy);
         const Mat x = s[0].defined() ? as_rows(s[0]) : Mat();
         NormGrads g = norm_backward(
-            x, {s[5], s[6]}, d, nullptr, contiguous_or_none(s[1]),
-            contiguous_or_none(s[2]), s[3], s[4], needs(ctx, 0),
+            x, {s[4], s[5]}, d, nullptr, contiguous_or_none(s[1]),
+            contiguous_or_none(s[2]), s[3], needs(ctx, 0),
             needs(ctx, 1) || needs(ctx, 2));
-        return {g.dx.defined() ? g.dx.view(dy.sizes()) : Tensor(), g.dgamma,
+        return {g.dx.defined() ? shaped(g.dx, dy.sizes()) : Tensor(), g.dgamma,
                 g.dbeta, Tensor(), Tensor()};
     }
 };
@@ -168,9 +173,9 @@ Tensor layer_norm(Tensor x, c10::optional<Tensor> weight,
         check_capture({x, gamma, beta});
         return NormFn::apply(x, maybe(gamma), maybe(beta), eps, act8);
     }
-    return norm_forward(as_rows(x), contiguous_or_none(gamma),
-                        contiguous_or_none(beta), eps, false, false, false,
-                        false).y.t.view(x.sizes());
+    return shaped(norm_forward(as_rows(x), contiguous_or_none(gamma),
+                               contiguous_or_none(beta), eps, false, false,
+                               false, false).y.t, x.sizes());
 }
 
 // ---- linear layer ----------------------------------------------------------------
@@ -201,7 +206,7 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
         ctx->saved_data["inputs"] = present({x, w, bias, res});
         ctx->saved_data["act"] = act;
         ctx->saved_data["how"] = (int64_t)o.u.how;
-        return o.y.t.view(out_sizes(x, w.size(0)));
+        return shaped(o.y.t, out_sizes(x, w.size(0)));
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -230,8 +235,9 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
                 db = row_sums(p, s[6].scalar_type());
             p.lo = Tensor();
             if (need_x)
-                dx = input_grad(p, as_rows(s[1]), 0, Kept(), Tensor(), nullptr,
-                                false).t.view(out_sizes(dy, s[1].size(1)));
+                dx = shaped(input_grad(p, as_rows(s[1]), 0, Kept(), Tensor(),
+                                       nullptr, false).t,
+                            out_sizes(dy, s[1].size(1)));
         }
         return {dx, dw, db, needs(ctx, 3) ? dy : Tensor(),
                 Tensor(), Tensor()};
@@ -259,10 +265,11 @@ Tensor linear_act(Tensor x, Tensor weight, c10::optional<Tensor> bias,
     }
     Mat rm;
     if (r.defined()) rm = as_rows(r);
-    return linear_forward(as_rows(x), as_rows(weight), contiguous_or_none(b),
-                          r.defined() ? &rm : nullptr, (int)act, false, false,
-                          false, false)
-        .y.t.view(out_sizes(x, weight.size(0)));
+    return shaped(linear_forward(as_rows(x), as_rows(weight),
+                                 contiguous_or_none(b),
+                                 r.defined() ? &rm : nullptr, (int)act, false,
+                                 false, false, false).y.t,
+                  out_sizes(x, weight.size(0)));
 }
 
 // ---- the block ---------------------------------------------------------------------
@@ -287,12 +294,11 @@ struct BlockFn : public torch::autograd::Function<BlockFn> {
         ctx->save_for_backward(
             {act8 ? none : x, act8 ? none : n.y.t, act8 ? none : a.y.t, n.x8.codes,
              n.x8.scales, n.y8.codes, n.y8.scales, a.y8.codes, a.y8.scales,
-             a.u.data, a.u.scales, n.mean, n.rstd, gamma, beta, w1, b1, w2,
-             b2});
+             a.u.data, a.u.scales, n.stats, gamma, beta, w1, b1, w2, b2});
         ctx->saved_data["inputs"] = present({x, gamma, beta, w1, b1, w2, b2});
         ctx->saved_data["act"] = act;
         ctx->saved_data["how"] = (int64_t)a.u.how;
-        return o.y.t.view(x.sizes());
+        return shaped(o.y.t, x.sizes());
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -302,7 +308,7 @@ struct BlockFn : public torch::autograd::Function<BlockFn> {
         const at::DeviceGuard guard(dy.device());
         const auto type = dy.scalar_type();
         const Mat d = as_rows(dy);
-        const Tensor &w1 = s[15], &b1 = s[16], &w2 = s[17], &b2 = s[18];
+        const Tensor &w1 = s[14], &b1 = s[15], &w2 = s[16], &b2 = s[17];
         auto need = [&](int i) { return needs(ctx, i); };
         auto kept = [&](int plain, int packed) {
             return s[plain].defined()
@@ -331,10 +337,10 @@ struct BlockFn : public torch::autograd::Function<BlockFn> {
                                           nullptr, false);
                 g = norm_backward(
                     s[0].defined() ? as_rows(s[0]) : Mat(), {s[3], s[4]},
-                    dh, &d, contiguous_or_none(s[13]),
-                    contiguous_or_none(s[14]), s[11], s[12], need(0),
+                    dh, &d, contiguous_or_none(s[12]),
+                    contiguous_or_none(s[13]), s[11], need(0),
                     need(1) || need(2));
-                if (need(0)) dx = g.dx.view(dy.sizes());
+                if (need(0)) dx = shaped(g.dx, dy.sizes());
             }
             if (!act8) p.lo = Tensor();
             if (need(3))
@@ -374,8 +380,8 @@ Tensor ffn_block(Tensor x, c10::optional<Tensor> norm_weight,
     const LinearOut a = linear_forward(n.y, as_rows(w1), contiguous_or_none(c1),
                                        nullptr, (int)act, false, false, false,
                                        true);
-    return linear_forward(a.y, as_rows(w2), contiguous_or_none(c2), &m, 0,
-                          false, false, false, false).y.t.view(x.sizes());
+    return shaped(linear_forward(a.y, as_rows(w2), contiguous_or_none(c2), &m, 0,
+                                 false, false, false, false).y.t, x.sizes());
 }
 
 // ---- the 8-bit form ------------------------------------------------------------------

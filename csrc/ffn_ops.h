@@ -34,7 +34,8 @@ struct Kept {
 void check_params(const at::Tensor& x, const at::Tensor& p, long long n,
                   const char* name);
 
-struct NormOut { Mat y; at::Tensor mean, rstd; Packed x8, y8; };
+// stats: [2, rows], the means and the 1 / deviations
+struct NormOut { Mat y; at::Tensor stats; Packed x8, y8; };
 NormOut norm_forward(const Mat& x, const at::Tensor& gamma,
                      const at::Tensor& beta, double eps, bool stats,
                      bool keep_x8, bool keep_y8, bool lines);
@@ -42,8 +43,8 @@ struct NormGrads { at::Tensor dx, dgamma, dbeta; };
 // x or, where it is defined, x8; `add` (or nothing) goes onto dx
 NormGrads norm_backward(const Mat& x, const Packed& x8, const Mat& dy,
                         const Mat* add, const at::Tensor& gamma,
-                        const at::Tensor& beta, const at::Tensor& mean,
-                        const at::Tensor& rstd, bool need_dx, bool need_params);
+                        const at::Tensor& beta, const at::Tensor& stats,
+                        bool need_dx, bool need_params);
 
 struct LinearOut { Mat y; Kept u; Packed y8; };
 LinearOut linear_forward(const Mat& x, const Mat& w, const at::Tensor& bias,

@@ -160,11 +160,8 @@ NormOut norm_forward(const Mat& x, const at::Tensor& gamma,
         o.y.rows = x.rows;
         o.y.dim = o.y.ld = x.dim;
     }
-    const auto f32 = x.t.options().dtype(at::kFloat);
-    if (stats) {
-        o.mean = at::empty({x.rows}, f32);
-        o.rstd = at::empty({x.rows}, f32);
-    }
+    if (stats)
+        o.stats = at::empty({2, x.rows}, x.t.options().dtype(at::kFloat));
     if (keep_x8) o.x8 = empty_packed(x.rows, x.dim, x.t);
     if (keep_y8) o.y8 = empty_packed(x.rows, x.dim, x.t);
     if (!x.rows) return o;
@@ -178,8 +175,8 @@ NormOut norm_forward(const Mat& x, const at::Tensor& gamma,
     a.y = o.y.t.data_ptr();
     a.ld_y = o.y.ld;
     if (stats) {
-        a.mean = o.mean.data_ptr<float>();
-        a.rstd = o.rstd.data_ptr<float>();
+        a.mean = o.stats.data_ptr<float>();
+        a.rstd = a.mean + x.rows;
     }
     if (keep_x8) {
         a.x8 = (signed char*)o.x8.codes.data_ptr();
@@ -225,9 +222,8 @@ static void sum_columns(const at::Tensor& part, long long n, long long width,
 
 NormGrads norm_backward(const Mat& x, const Packed& x8, const Mat& dy,
                         const Mat* add, const at::Tensor& gamma,
-                        const at::Tensor& beta, const at::Tensor& mean,
-                        const at::Tensor& rstd, bool need_dx,
-                        bool need_params) {
+                        const at::Tensor& beta, const at::Tensor& stats,
+                        bool need_dx, bool need_params) {
     const long long rows = dy.rows, dim = dy.dim;
     NormGrads g;
     if (need_dx) g.dx = at::empty({rows, dim}, dy.t.options());
@@ -255,8 +251,8 @@ NormGrads norm_backward(const Mat& x, const Packed& x8, const Mat& dy,
     }
     a.gamma = gamma.defined() ? gamma.data_ptr() : nullptr;
     a.p32 = gamma.defined() && gamma.scalar_type() == at::kFloat;
-    a.mean = mean.data_ptr<float>();
-    a.rstd = rstd.data_ptr<float>();
+    a.mean = stats.data_ptr<float>();
+    a.rstd = a.mean + rows;
     a.dx = need_dx ? g.dx.data_ptr() : nullptr;
     a.rows = (int)rows;
     a.dim = (int)dim;
