@@ -81,7 +81,9 @@ __device__ __forceinline__ float norm_rstd(float q, float more, float n,
 
 // A team of NT threads takes a row at a time and holds it in registers, R
 // chunks of 8 a thread: x is read once, the mean comes first and the variance
-// from what is left of it.
+// from what is left of it.  Bound by memory: 32768 x 2048 in fp32 99 us (5.4
+// TB/s), and nearly so by instructions in 16 bits with the 8-bit form: 17920 x
+// 1500 32 us (4.2 TB/s).
 template <typename T, int NT, int R>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_forward_kernel(
         NormArgs p) {
@@ -227,7 +229,8 @@ __device__ __forceinline__ void load_kept(const NormGradArgs& p, long long row,
 // dx = rstd (g dy - mean(g dy) - xh mean(g dy xh)).  x and dy are read once;
 // each thread sums dy xh and dy for its own columns over the rows that it
 // sees, the teams of a block add theirs in turn, and column_sum_kernel adds
-// the blocks': no atomics, the same result each time.
+// the blocks': no atomics, the same result each time.  32768 x 2048 in fp32 151
+// us (5.3 TB/s).
 template <typename T, int NT, int R, bool X8>
 __global__ __launch_bounds__(NT < 128 ? 256 : NT) void norm_backward_kernel(
         NormGradArgs p) {
@@ -483,7 +486,7 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(
 // ---- the 8-bit form by itself ------------------------------------------------------
 // A group of 128 values for each 16 lanes, GROUPS of them at a time; I is the
 // type that counts them.  17920 x 6000 in bf16, us: one group 66, two 64, four
-// 66, and 74 with a quarter of the blocks.
+// 66, and 74 with a quarter of the blocks; in a step, from memory, 77 (4.2 TB/s).
 template <typename T, typename I>
 __global__ __launch_bounds__(256) void act8_pack_kernel(
         const T* x, long long ld, I rows, int dim, signed char* codes,
@@ -515,7 +518,8 @@ __global__ __launch_bounds__(256) void act8_pack_kernel(
 }
 
 // Values of 8 bits to 16 or 32, rows ld apart, a chunk of 8 a thread: 17920 x 6000
-// to fp32 93 us; with two to eight chunks a thread 115 to 137.
+// to fp32 93 us, with two to eight chunks a thread 115 to 137; in a step, from
+// memory, 105 (5.1 TB/s).
 template <typename O, typename I>
 __global__ __launch_bounds__(256) void act8_unpack_kernel(
         const signed char* codes, const float* scales, I rows, int dim, O* out,
