@@ -391,7 +391,7 @@ std::vector<Tensor> act8_pack(Tensor x) {
     const Packed p = pack(as_rows(x));
     std::vector<int64_t> s = x.sizes().vec();
     s.back() = p.scales.size(1);
-    return {p.codes.view(x.sizes()), p.scales.view(s)};
+    return {shaped(p.codes, x.sizes()), shaped(p.scales, s)};
 }
 
 Tensor act8_unpack(Tensor codes, Tensor scales, int64_t type) {
@@ -414,9 +414,9 @@ Tensor act8_unpack(Tensor codes, Tensor scales, int64_t type) {
     const auto t = type == 0 ? at::kFloat : type == 1 ? at::kBFloat16
                                                       : at::kHalf;
     const int64_t rows = codes.numel() / dim;
-    return unpack(codes.contiguous().view({rows, dim}),
-                  scales.contiguous().view({rows, s.back()}), t, false)
-        .t.view(codes.sizes());
+    return shaped(unpack(shaped(codes.contiguous(), {rows, dim}),
+                         shaped(scales.contiguous(), {rows, s.back()}), t,
+                         false).t, codes.sizes());
 }
 
 }  // namespace ffn

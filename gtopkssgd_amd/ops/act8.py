@@ -46,7 +46,7 @@ def act8_pack(x: torch.Tensor) -> Act8:
     """The 8-bit form of ``x`` (bf16, fp16 or fp32), by groups of its last
     dimension.  Not differentiable."""
     if x.is_cuda:
-        return Act8(*_ext().act8_pack(x.detach()))
+        return Act8(*_ext().act8_pack(x))
     if x.dim() < 1 or x.size(-1) == 0 or not x.is_floating_point():
         raise RuntimeError("act8_pack needs floating values with a last "
                            f"dimension, got {x.dtype} {tuple(x.shape)}")

@@ -370,6 +370,16 @@ def test_act8_edges_are_the_cpu_ones():
     assert torch.equal(p.scales.cpu().nan_to_num(-1), q.scales.nan_to_num(-1))
 
 
+@pytest.mark.parametrize("shape", [(5, 200), (3, 2, 200), (200,)])
+def test_act8_pack_of_a_leaf_is_not_differentiable(shape):
+    x = make(*shape).transpose(0, -1) if len(shape) > 2 else make(*shape)
+    p = gt.act8_pack(x)
+    assert not p.codes.requires_grad and not p.scales.requires_grad
+    assert p.scales.grad_fn is None
+    back = gt.act8_unpack(*p)
+    assert back.shape == x.shape and not back.requires_grad
+
+
 def test_act8_more_chunks_than_threads():
     """9 rows of 2^30 - 8 values: more chunks of 8 than one launch has threads
     for, the last of them against the codes."""
