@@ -556,6 +556,89 @@ def test_same_bits_each_time(act8, t, rows, d, h):
     assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
+@pytest.mark.parametrize("rows", [5, 90])
+def test_one_tensor_twice(rows):
+    """x as its own residual and weight: both edges get their gradients."""
+    v = make(rows, rows, t=FP, scale=0.3)
+    a, b, c = (v.detach().clone().requires_grad_() for _ in range(3))
+    dy = make(rows, rows, t=FP, seed=3, grad=False)
+    once = torch.autograd.grad(
+        gt.linear_act(v, v, None, v, act="silu"), v, dy)[0]
+    parts = torch.autograd.grad(
+        gt.linear_act(a, b, None, c, act="silu"), (a, b, c), dy)
+    # two additions of three values in fp32
+    bound = sum(p.abs() for p in parts) * 2 ** -22
+    assert bool(((once - sum(parts)).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("act8", [False, True])
+@pytest.mark.parametrize("rows", [3, 150])
+def test_block_gradients_that_are_no_plain_tensor(act8, rows):
+    """A gradient expanded from one value, a transposed one, a graph kept for a
+    second pass, and gradients that add up."""
+    args = block_args(rows, 72, 200, BF)
+    y = gt.ffn_block(*args, act8=act8)
+    flat = torch.autograd.grad(y, args, torch.ones_like(y), retain_graph=True)
+    wide = torch.autograd.grad(y, args, y.new_ones(()).expand(y.shape),
+                               retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(flat, wide))
+    dy = make(72, rows, t=BF, seed=8, grad=False)
+    turned = torch.autograd.grad(y, args, dy.t(), retain_graph=True)
+    whole = torch.autograd.grad(y, args, dy.t().contiguous(),
+                                retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(turned, whole))
+    y.backward(dy.t(), retain_graph=True)
+    assert all(torch.equal(p.grad, b) for p, b in zip(args, whole))
+    y.backward(dy.t())
+    for p, b in zip(args, whole):
+        assert torch.equal(p.grad, 2 * b)
+
+
+@pytest.mark.parametrize("rows", [7, 200])
+@pytest.mark.parametrize("t", [BF, HF, FP])
+def test_block_parameters_out_of_one_buffer(rows, t):
+    """Parameters at every alignment that the type allows, as views of one flat
+    buffer are."""
+    args = block_args(rows, 39, 77, t)
+    dy = make(rows, 39, t=t, seed=8, grad=False)
+    want = torch.autograd.grad(gt.ffn_block(*args), args, dy)
+    size = sum(a.numel() + 1 for a in args)
+    flat = torch.empty(size, dtype=t, device=DEV)
+    at, views = 1, []
+    for a in args:
+        v = flat[at:at + a.numel()].view(a.shape)
+        v.copy_(a.detach())
+        views.append(v.detach().requires_grad_())
+        at += a.numel() + 1
+    got = torch.autograd.grad(gt.ffn_block(*views), views, dy)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_two_threads_at_once():
+    import threading
+    args = [block_args(rows, 72, 200, BF) for rows in (40, 300)]
+    dys = [torch.ones_like(a[0]) for a in args]
+    want = [torch.autograd.grad(gt.ffn_block(*a, act8=True), a, dy)
+            for a, dy in zip(args, dys)]
+    got = [None, None]
+    torch.cuda.synchronize()
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                got[i] = torch.autograd.grad(
+                    gt.ffn_block(*args[i], act8=True), args[i], dys[i])
+        s.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 def test_other_stream():
     args = block_args(300, 200, 400, BF)
     dy = make(300, 200, t=BF, seed=9, grad=False)
