@@ -190,18 +190,22 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
                           const Tensor& w, const Maybe& maybe_bias,
                           const Maybe& maybe_res, int64_t act, bool act8) {
         const Tensor bias = or_none(maybe_bias), res = or_none(maybe_res);
-        const Mat m = as_rows(x);
+        const Mat mx = as_rows(x), mw = as_rows(w);
+        const Mat m = on_lines(mx, mw.rows), wm = on_lines(mw, mx.rows);
         Mat r;
         if (res.defined()) r = as_rows(res);
         const bool through = wants_grad(x) || wants_grad(w) ||
                              wants_grad(bias);
-        LinearOut o = linear_forward(m, as_rows(w), contiguous_or_none(bias),
+        LinearOut o = linear_forward(m, wm, contiguous_or_none(bias),
                                      res.defined() ? &r : nullptr, (int)act,
                                      through, act8, false, false);
         Packed x8;
         if (wants_grad(w) && act8) x8 = pack(m);
-        ctx->save_for_backward({wants_grad(w) && !act8 ? x : Tensor(),
-                                wants_grad(x) ? w : Tensor(), x8.codes,
+        // a copy that was made serves the backward pass too
+        const Tensor& kept_x = m.t.is_same(mx.t) ? x : m.t;
+        const Tensor& kept_w = wm.t.is_same(mw.t) ? w : wm.t;
+        ctx->save_for_backward({wants_grad(w) && !act8 ? kept_x : Tensor(),
+                                wants_grad(x) ? kept_w : Tensor(), x8.codes,
                                 x8.scales, o.u.data, o.u.scales, bias});
         ctx->saved_data["inputs"] = present({x, w, bias, res});
         ctx->saved_data["act"] = act;
@@ -264,8 +268,10 @@ Tensor linear_act(Tensor x, Tensor weight, c10::optional<Tensor> bias,
         return LinearFn::apply(x, weight, maybe(b), maybe(r), act, act8);
     }
     Mat rm;
+    const Mat m = as_rows(x);
     if (r.defined()) rm = as_rows(r);
-    return shaped(linear_forward(as_rows(x), as_rows(weight),
+    return shaped(linear_forward(on_lines(m, weight.size(0)),
+                                 on_lines(as_rows(weight), m.rows),
                                  contiguous_or_none(b),
                                  r.defined() ? &rm : nullptr, (int)act, false,
                                  false, false, false).y.t,
@@ -285,16 +291,20 @@ struct BlockFn : public torch::autograd::Function<BlockFn> {
         NormOut n = norm_forward(m, contiguous_or_none(gamma),
                                  contiguous_or_none(beta), eps, true, act8,
                                  act8, true);
-        LinearOut a = linear_forward(n.y, as_rows(w1), contiguous_or_none(b1),
-                                     nullptr, (int)act, true, act8, act8,
-                                     true);
-        LinearOut o = linear_forward(a.y, as_rows(w2), contiguous_or_none(b2),
-                                     &m, 0, false, false, false, false);
+        const Mat r1 = as_rows(w1), r2 = as_rows(w2);
+        const Mat m1 = on_lines(r1, m.rows), m2 = on_lines(r2, m.rows);
+        LinearOut a = linear_forward(n.y, m1, contiguous_or_none(b1), nullptr,
+                                     (int)act, true, act8, act8, true);
+        LinearOut o = linear_forward(a.y, m2, contiguous_or_none(b2), &m, 0,
+                                     false, false, false, false);
+        const Tensor& kept1 = m1.t.is_same(r1.t) ? w1 : m1.t;
+        const Tensor& kept2 = m2.t.is_same(r2.t) ? w2 : m2.t;
         const Tensor none;
         ctx->save_for_backward(
             {act8 ? none : x, act8 ? none : n.y.t, act8 ? none : a.y.t, n.x8.codes,
              n.x8.scales, n.y8.codes, n.y8.scales, a.y8.codes, a.y8.scales,
-             a.u.data, a.u.scales, n.stats, gamma, beta, w1, b1, w2, b2});
+             a.u.data, a.u.scales, n.stats, gamma, beta, kept1, b1, kept2,
+             b2});
         ctx->saved_data["inputs"] = present({x, gamma, beta, w1, b1, w2, b2});
         ctx->saved_data["act"] = act;
         ctx->saved_data["how"] = (int64_t)a.u.how;
@@ -377,11 +387,12 @@ Tensor ffn_block(Tensor x, c10::optional<Tensor> norm_weight,
     const NormOut n = norm_forward(m, contiguous_or_none(gamma),
                                    contiguous_or_none(beta), eps, false, false,
                                    false, true);
-    const LinearOut a = linear_forward(n.y, as_rows(w1), contiguous_or_none(c1),
-                                       nullptr, (int)act, false, false, false,
-                                       true);
-    return shaped(linear_forward(a.y, as_rows(w2), contiguous_or_none(c2), &m, 0,
-                                 false, false, false, false).y.t, x.sizes());
+    const LinearOut a = linear_forward(n.y, on_lines(as_rows(w1), m.rows),
+                                       contiguous_or_none(c1), nullptr,
+                                       (int)act, false, false, false, true);
+    return shaped(linear_forward(a.y, on_lines(as_rows(w2), m.rows),
+                                 contiguous_or_none(c2), &m, 0, false, false,
+                                 false, false).y.t, x.sizes());
 }
 
 // ---- the 8-bit form ------------------------------------------------------------------

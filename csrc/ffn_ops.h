@@ -24,6 +24,10 @@ Mat unpack(const at::Tensor& codes, const at::Tensor& scales,
 Mat empty_rows(long long rows, long long dim, const at::Tensor& like,
                at::ScalarType type);
 
+// m, or a copy whose rows start on lines where a product with `other` rows or
+// columns gains more by them than the copy takes
+Mat on_lines(const Mat& m, long long other);
+
 // what the backward pass sees of a value: itself, its 8-bit form, or for relu
 // the sign in bits
 struct Kept {

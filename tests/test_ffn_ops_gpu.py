@@ -194,6 +194,52 @@ def test_linear_bias_gradient_beside_the_weights(k, m, n, t, bias):
     linear_case(m, k, n, t, bias=bias)
 
 
+def on_lines(v):
+    ld = -(-v.shape[1] // 64) * 64
+    out = torch.full((v.shape[0], ld), float("nan"), dtype=v.dtype, device=DEV)
+    out = out[:, :v.shape[1]]
+    out.copy_(v.detach())
+    return out.requires_grad_(v.requires_grad)
+
+
+@pytest.mark.parametrize("t", [BF, HF])
+@pytest.mark.parametrize("act,act8", [("none", False), ("gelu", True)])
+def test_linear_copies_long_operands(t, act, act8):
+    """Operands that are copied to rows on lines: the same bits as from operands
+    that lie so, and some rows against 64 bits."""
+    m, k, n = 20000, 499, 20100
+    x, w = make(m, k, t=t), make(n, k, t=t, scale=k ** -0.5, seed=1)
+    b = make(n, t=t, seed=2)
+    dy = make(m, n, t=t, seed=3, grad=False)
+    got = gt.linear_act(x, w, b, act=act, act8=act8)
+    lines = [on_lines(x), on_lines(w), b]
+    want = gt.linear_act(*lines, act=act, act8=act8)
+    assert torch.equal(got, want)
+    with torch.no_grad():
+        assert torch.equal(gt.linear_act(x, w, b, act=act), want)
+    rows = [0, 1, 777, m - 1]
+    sample = ref.linear(ref.wide(x[rows]), ref.wide(w), ref.wide(b), None, act,
+                        t, act8, ref.wide(dy[rows]))
+    ref.close(got[rows], *sample[0], what="y")
+    got = torch.autograd.grad(got, [x, w, b], dy)
+    want = torch.autograd.grad(want, lines, dy)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    ref.close(got[0][rows], *sample[1], what="dx")
+
+
+def test_block_copies_long_weights():
+    args = block_args(20000, 499, 9001, BF)
+    dy = make(20000, 499, t=BF, seed=9, grad=False)
+    lines = list(args)
+    lines[3], lines[5] = on_lines(args[3]), on_lines(args[5])
+    ys = [gt.ffn_block(*a, act8=True) for a in (args, lines)]
+    assert torch.equal(*ys)
+    with torch.no_grad():
+        assert torch.equal(gt.ffn_block(*args), ys[0])
+    got, want = (torch.autograd.grad(y, a, dy) for y, a in zip(ys, (args, lines)))
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
 @pytest.mark.parametrize("m,k,n", [(2500, 300, 40), (40, 3100, 70),
                                    (70, 50, 2500), (2100, 520, 530)])
 @pytest.mark.parametrize("t", [BF, FP])
