@@ -227,6 +227,27 @@ def test_linear_copies_long_operands(t, act, act8):
     ref.close(got[0][rows], *sample[1], what="dx")
 
 
+@pytest.mark.parametrize("m,k,n", [(8000, 2570, 2900), (20001, 1500, 2000),
+                                   (30000, 1023, 777), (12345, 256, 4100),
+                                   (9000, 3900, 3900)])
+@pytest.mark.parametrize("t", [BF, HF])
+def test_linear_long_weight_gradients(m, k, n, t):
+    """Sums over many rows, whole and in parts, against 64 bits: half a step of
+    rounding, and the rounding of m additions in fp32."""
+    x = make(m, k, t=t, grad=False)
+    w, b = make(n, k, t=t, seed=1), make(n, t=t, seed=2)
+    dy = make(m, n, t=t, seed=3, grad=False)
+    dw, db = torch.autograd.grad(gt.linear_act(x, w, b), [w, b], dy)
+    xd, d = x.double(), dy.double().t().contiguous()
+    for got, one in ((dw, xd), (db[:, None], torch.ones_like(xd[:, :1]))):
+        want = torch.mm(d, one)
+        bound = want.abs() * torch.finfo(t).eps / 2 + \
+            torch.mm(d.abs(), one.abs()) * m * 2.0 ** -24 + 2.0 ** -24
+        assert bool(((got.double() - want).abs() <= bound).all())
+    again = torch.autograd.grad(gt.linear_act(x, w, b), [w, b], dy)
+    assert torch.equal(again[0], dw) and torch.equal(again[1], db)
+
+
 def test_block_copies_long_weights():
     args = block_args(20000, 499, 9001, BF)
     dy = make(20000, 499, t=BF, seed=9, grad=False)
