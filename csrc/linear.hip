@@ -321,7 +321,7 @@ Mat input_grad(const Mat& p, const Mat& w, int act, const Kept& u,
 }
 
 // The sum of p's rows is a column of ones on x, where the last tile has room for
-// it: by itself it reads p once more, at 17920 x 10000 in bf16 97 of 1780 us.
+// it: by itself it reads p once more, at 17920 x 10000 in bf16 97 us beside 450.
 at::Tensor weight_grad(const Mat& p, const Mat& x, const at::Tensor& bias,
                        at::Tensor* dbias) {
     auto out = at::empty({p.dim, x.dim}, p.t.options());
