@@ -192,7 +192,8 @@ struct Operand {
 
 // ---- block index -> output tile ---------------------------------------------
 // Blocks go round the 8 dies in turn; each die gets neighbouring tiles, 8 tile
-// rows by all columns at a time, so that its L2 holds what they share.
+// rows by all columns at a time, so that its L2 holds what they share (4 or 16
+// rows: 1 % slower over a block's training step of 17920 rows).
 __device__ __forceinline__ void tile_of(int bid, int tm, int tn, int* m,
                                         int* n) {
     const int nb = tm * tn, x = bid & 7;

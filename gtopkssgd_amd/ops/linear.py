@@ -7,7 +7,9 @@ and its backward pass (csrc/linear.hip).
 
 For the backward pass the layer keeps x, W and, for gelu and silu, u; relu
 keeps one bit a value.  ``act8=True`` keeps x and u in 8 bits (``act8``
-module): half the memory, and gradients from what those stand for.
+module): half the memory, and gradients from what those stand for.  On the GPU
+long 16-bit operands of wide products are copied to rows that start on lines of
+128 bytes, and the backward pass uses the copy.
 """
 from __future__ import annotations
 

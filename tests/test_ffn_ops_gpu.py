@@ -756,6 +756,38 @@ def test_captured_steps():
                 assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("m,k,n,t", [(1, 100, 300, BF), (20, 1500, 700, HF),
+                                     (33, 77, 50, FP), (20000, 499, 20100, BF)])
+def test_captured_linear_layers(m, k, n, t):
+    """Few rows, and operands that are copied to rows on lines: every replay
+    against the eager result, with eager work between."""
+    x, w = make(m, k, t=t), make(n, k, t=t, scale=k ** -0.5, seed=1)
+    b, g = make(n, t=t, seed=2), make(k, t=t, seed=4)
+    dy = make(m, n, t=t, seed=3, grad=False)
+
+    def step():
+        with torch.no_grad():
+            plain = gt.linear_act(gt.layer_norm(x, g), w, b, act="silu")
+        y = gt.linear_act(x, w, b)
+        return [plain, y.detach(), *torch.autograd.grad(y, (x, w, b), dy)]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for turn in range(3):
+        with torch.no_grad():
+            x.add_(0.25 * turn)
+            w.mul_(1.0 + 0.5 * turn)
+        want = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(outs, want))
+
+
 @pytest.mark.parametrize("which", ["norm", "linear", "block"])
 def test_capture_refuses_a_living_graph_of_its_leaves(which):
     args = block_args(40, 24, 56, BF)
