@@ -122,15 +122,14 @@ __device__ __forceinline__ void store8(T* p, int left, const float* v) {
 }
 
 __device__ __forceinline__ void load8_codes(const signed char* p, int left,
-                                            float scale, float* v) {
+                                            float* v) {
     if (left >= 8) {
         const i8x8 c = *reinterpret_cast<const i8x8*>(p);
         #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (float)c[i] * scale;
+        for (int i = 0; i < 8; ++i) v[i] = (float)c[i];
     } else {
         #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] = i < left ? (float)p[i] * scale : 0.0f;
+        for (int i = 0; i < 8; ++i) v[i] = i < left ? (float)p[i] : 0.0f;
     }
 }
 

@@ -183,7 +183,10 @@ template <typename T, bool X8> struct KeptRaw {
                                            float* v) const {
         unpack8(raw, c, dim, whole, v);
     }
-    __device__ __forceinline__ float by(float rstd) const { return rstd; }
+    // x - mean, of what unpack() brought
+    __device__ __forceinline__ float from(float v, float mean) const {
+        return v - mean;
+    }
 };
 template <typename T> struct KeptRaw<T, true> {
     u32x2 raw;
@@ -209,21 +212,25 @@ template <typename T> struct KeptRaw<T, true> {
                                            float* v) const {
         unpack8(__builtin_bit_cast(i8x8, raw), c, dim, whole, v);
     }
-    // what a code is multiplied by
-    __device__ __forceinline__ float by(float rstd) const {
-        return scale * rstd;
+    __device__ __forceinline__ float from(float v, float mean) const {
+        return __builtin_fmaf(v, scale, -mean);
     }
 };
 
+// x - mean for 8 columns of the kept x, from c on
 template <typename T>
 __device__ __forceinline__ void load_kept(const NormGradArgs& p, long long row,
-                                          int c, int left, float* v) {
-    if (p.x8)
-        load8_codes(p.x8 + row * p.dim + c, left,
-                    left > 0 ? p.x8_scale[row * groups_of(p.dim) +
-                                          c / ACT8_GROUP] : 0.0f, v);
-    else
+                                          int c, int left, float mean,
+                                          float* v) {
+    float scale = 1.0f;
+    if (p.x8) {
+        load8_codes(p.x8 + row * p.dim + c, left, v);
+        scale = p.x8_scale[row * groups_of(p.dim) + c / ACT8_GROUP];
+    } else {
         load8((const T*)p.x + row * p.ld + c, left, v);
+    }
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __builtin_fmaf(v[i], scale, -mean);
 }
 
 // dx = rstd (g dy - mean(g dy) - xh mean(g dy xh)).  x and dy are read once;
@@ -260,20 +267,20 @@ __global__ __launch_bounds__(NT < 128 ? 256 : NT) void norm_backward_kernel(
             rh[i].fetch(p, row, c);
             rd[i] = fetch8((const T*)p.dy + row * p.ld_dy, c, p.dim);
         }
-        // xh = x rstd - mean rstd, a code times its scale and rstd; columns that
-        // are not there have dy = 0
+        // xh = (x - mean) rstd, x a code times its scale: the difference first,
+        // since products with rstd round by steps of x, and in a row far from 0
+        // for its spread nothing else would be left of xh.  Columns that are not
+        // there have dy = 0.
         float h[R][8], d[R][8];
-        const float shift = -mean * rstd;
         #pragma unroll
         for (int i = 0; i < R; ++i) {
             const int c = (i * NT + t) * 8;
             const bool whole = (i + 1) * NT * 8 <= p.dim;
             rh[i].unpack(c, p.dim, whole, h[i]);
             unpack8(rd[i], c, p.dim, whole, d[i]);
-            const float by = rh[i].by(rstd);
             #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                h[i][j] = __builtin_fmaf(h[i][j], by, shift);
+                h[i][j] = rh[i].from(h[i][j], mean) * rstd;
                 sg[i][j] = __builtin_fmaf(d[i][j], h[i][j], sg[i][j]);
                 sb[i][j] += d[i][j];
                 d[i][j] *= g[i][j];
@@ -387,13 +394,13 @@ __global__ __launch_bounds__(1024) void norm_dx_wide_kernel(NormGradArgs p) {
     const float mean = p.mean[row], rstd = p.rstd[row];
     float s1 = 0.0f, s2 = 0.0f, h[8], d[8], g[8], a[8];
     for (int c = threadIdx.x * 8; c < p.dim; c += step) {
-        load_kept<T>(p, row, c, p.dim - c, h);
+        load_kept<T>(p, row, c, p.dim - c, mean, h);
         load8((const T*)p.dy + row * p.ld_dy + c, p.dim - c, d);
         load_param<T>(p.gamma, p.p32, c, p.dim - c, 1.0f, g);
         #pragma unroll
         for (int j = 0; j < 8; ++j) {
             s1 += d[j] * g[j];
-            s2 += d[j] * g[j] * (h[j] - mean) * rstd;
+            s2 += d[j] * g[j] * h[j] * rstd;
         }
     }
     team_sum2<1024>(s1, s2, slots);
@@ -401,14 +408,13 @@ __global__ __launch_bounds__(1024) void norm_dx_wide_kernel(NormGradArgs p) {
     s2 /= p.dim;
     for (int c = threadIdx.x * 8; c < p.dim; c += step) {
         const int left = p.dim - c;
-        load_kept<T>(p, row, c, left, h);
+        load_kept<T>(p, row, c, left, mean, h);
         load8((const T*)p.dy + row * p.ld_dy + c, left, d);
         load_param<T>(p.gamma, p.p32, c, left, 1.0f, g);
         if (p.add) load8((const T*)p.add + row * p.ld_add + c, left, a);
         #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float v = rstd * (d[j] * g[j] - s1 -
-                                    (h[j] - mean) * rstd * s2);
+            const float v = rstd * (d[j] * g[j] - s1 - h[j] * rstd * s2);
             d[j] = p.add ? v + a[j] : v;
         }
         store8((T*)p.dx + (long long)row * p.dim + c, left, d);
@@ -435,10 +441,10 @@ __global__ __launch_bounds__(256) void row_sum_kernel(NormGradArgs p,
             unpack8(fetch8((const T*)p.dy + row * p.ld_dy, c, p.dim), c, p.dim,
                     whole, d);
             if (NORM) {
-                load_kept<T>(p, row, c, left, h);
+                load_kept<T>(p, row, c, left, p.mean[row], h);
                 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    sg[j] += d[j] * (h[j] - p.mean[row]) * p.rstd[row];
+                    sg[j] += d[j] * h[j] * p.rstd[row];
             }
             #pragma unroll
             for (int j = 0; j < 8; ++j) sb[j] += d[j];
