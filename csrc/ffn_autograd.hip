@@ -2,8 +2,10 @@
 // is kept for the backward pass, and the backward pass itself.
 #include "ffn_ops.h"
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 namespace ffn {
 
@@ -59,6 +61,29 @@ static void check_norm_params(const Tensor& x, const Tensor& gamma,
 
 static void check_act(int64_t act) {
     TORCH_CHECK(act >= 0 && act <= 3, "no activation ", act);
+}
+
+// The kernels are launched past torch's dispatcher.  What follows a call there
+// would see no more of it than the allocation of its result: a derivative of
+// zero in forward mode, a graph without the kernel.
+static void check_seen(const char* name, std::initializer_list<Tensor> all) {
+    using Modes = c10::impl::TorchDispatchModeTLS;
+    using Mode = c10::impl::TorchDispatchModeKey;
+    TORCH_CHECK(!torch::jit::tracer::isTracing() &&
+                !Modes::get_mode(Mode::PROXY) && !Modes::get_mode(Mode::FAKE) &&
+                !Modes::get_mode(Mode::FUNCTIONAL),
+                name, " cannot be traced: its kernels are no operators of torch");
+    for (const Tensor& t : all) {
+        if (!t.defined()) continue;
+        TORCH_CHECK(t.has_storage() &&
+                    !t.unsafeGetTensorImpl()->key_set().has_any(
+                        c10::DispatchKeySet({c10::DispatchKey::FuncTorchBatched,
+                            c10::DispatchKey::FuncTorchGradWrapper,
+                            c10::DispatchKey::Functionalize})),
+                    name, " has no form for the transforms of torch.func");
+        TORCH_CHECK(!t._fw_grad(0).defined(), name,
+                    " has no derivative in forward mode");
+    }
 }
 
 static bool wants_grad(const Tensor& t) {
@@ -164,6 +189,7 @@ struct NormFn : public torch::autograd::Function<NormFn> {
 Tensor layer_norm(Tensor x, c10::optional<Tensor> weight,
                   c10::optional<Tensor> bias, double eps, bool act8) {
     const Tensor gamma = or_none(weight), beta = or_none(bias);
+    check_seen("layer_norm", {x, gamma, beta});
     check_values(x, "x");
     check_norm_params(x, gamma, beta, "weight", "bias");
     TORCH_CHECK(x.size(-1) < (1LL << 25), "rows of ", x.size(-1),
@@ -251,6 +277,7 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
 Tensor linear_act(Tensor x, Tensor weight, c10::optional<Tensor> bias,
                   c10::optional<Tensor> residual, int64_t act, bool act8) {
     const Tensor b = or_none(bias), r = or_none(residual);
+    check_seen("linear_act", {x, weight, b, r});
     check_values(x, "x");
     check_weight(x, weight, x.size(-1), "weight");
     check_params(x, b, weight.size(0), "bias");
@@ -368,6 +395,7 @@ Tensor ffn_block(Tensor x, c10::optional<Tensor> norm_weight,
                  bool act8) {
     const Tensor gamma = or_none(norm_weight), beta = or_none(norm_bias);
     const Tensor c1 = or_none(b1), c2 = or_none(b2);
+    check_seen("ffn_block", {x, gamma, beta, w1, c1, w2, c2});
     check_values(x, "x");
     check_norm_params(x, gamma, beta, "norm_weight", "norm_bias");
     check_weight(x, w1, x.size(-1), "w1");
@@ -397,6 +425,7 @@ Tensor ffn_block(Tensor x, c10::optional<Tensor> norm_weight,
 
 // ---- the 8-bit form ------------------------------------------------------------------
 std::vector<Tensor> act8_pack(Tensor x) {
+    check_seen("act8_pack", {x});
     check_values(x, "x");
     const at::DeviceGuard guard(x.device());
     const Packed p = pack(as_rows(x));
@@ -406,6 +435,9 @@ std::vector<Tensor> act8_pack(Tensor x) {
 }
 
 Tensor act8_unpack(Tensor codes, Tensor scales, int64_t type) {
+    check_seen("act8_unpack", {codes, scales});
+    TORCH_CHECK(!recording({scales}), "act8_unpack has no gradient: scales must "
+                "not require one");
     TORCH_CHECK(codes.is_cuda() && scales.device() == codes.device(),
                 "codes and scales must be on one GPU, got ", codes.device(),
                 " and ", scales.device());

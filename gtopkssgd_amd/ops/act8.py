@@ -44,7 +44,8 @@ def _groups(x: torch.Tensor) -> torch.Tensor:
 
 def act8_pack(x: torch.Tensor) -> Act8:
     """The 8-bit form of ``x`` (bf16, fp16 or fp32), by groups of its last
-    dimension.  Not differentiable."""
+    dimension.  Not differentiable; on the GPU forward mode, torch.func's
+    transforms and tracing are refused."""
     if x.is_cuda:
         return Act8(*_ext().act8_pack(x))
     if x.dim() < 1 or x.size(-1) == 0 or not x.is_floating_point():
@@ -66,7 +67,9 @@ def act8_pack(x: torch.Tensor) -> Act8:
 
 def act8_unpack(codes: torch.Tensor, scales: torch.Tensor,
                 dtype: torch.dtype = torch.float32) -> torch.Tensor:
-    """The values that an 8-bit form stands for, rounded once to ``dtype``."""
+    """The values that an 8-bit form stands for, rounded once to ``dtype``.  On
+    the GPU scales that require a gradient are refused, and what ``act8_pack``
+    refuses."""
     if codes.is_cuda:
         if dtype not in _TYPES:
             raise RuntimeError(f"act8_unpack gives {list(_TYPES)}, "

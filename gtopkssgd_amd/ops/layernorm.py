@@ -61,7 +61,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     x: bf16, fp16 or fp32, any leading dimensions and strides.
     weight, bias: [x.size(-1)], both of x's type or both fp32; either may be
     None.  The result has x's type; statistics and sums are fp32.  No second
-    derivative."""
+    derivative; on the GPU forward mode, torch.func's transforms and tracing
+    are refused."""
     if x.is_cuda:
         return _ext().layer_norm(x, weight, bias, float(eps), bool(act8))
     if x.dim() < 1 or x.size(-1) == 0:

@@ -100,7 +100,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor,
     fp16 or fp32); bias: [out] of that type or fp32.  act: "none", "relu",
     "gelu" (the exact one) or "silu".  Sums are fp32, the result is rounded
     once.  Under autocast x, weight and residual are cast to its type.  No
-    second derivative."""
+    second derivative; on the GPU forward mode, torch.func's transforms and
+    tracing are refused."""
     code = _act_code(act)
     if x.is_cuda:
         if torch.is_autocast_enabled("cuda"):
