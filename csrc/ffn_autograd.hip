@@ -163,11 +163,11 @@ struct NormFn : public torch::autograd::Function<NormFn> {
         const Mat m = as_rows(x);
         NormOut o = norm_forward(m, contiguous_or_none(gamma),
                                  contiguous_or_none(beta), eps, true, act8,
-                                 false, false);
+                                 false, x.sizes());
         ctx->save_for_backward({act8 ? Tensor() : x, gamma, beta, o.stats,
                                 o.x8.codes, o.x8.scales});
         ctx->saved_data["inputs"] = present({x, gamma, beta});
-        return shaped(o.y.t, x.sizes());
+        return o.y.t;
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -180,9 +180,8 @@ struct NormFn : public torch::autograd::Function<NormFn> {
         NormGrads g = norm_backward(
             x, {s[4], s[5]}, d, nullptr, contiguous_or_none(s[1]),
             contiguous_or_none(s[2]), s[3], needs(ctx, 0),
-            needs(ctx, 1) || needs(ctx, 2));
-        return {g.dx.defined() ? shaped(g.dx, dy.sizes()) : Tensor(), g.dgamma,
-                g.dbeta, Tensor(), Tensor()};
+            needs(ctx, 1) || needs(ctx, 2), dy.sizes());
+        return {g.dx, g.dgamma, g.dbeta, Tensor(), Tensor()};
     }
 };
 
@@ -199,9 +198,9 @@ Tensor layer_norm(Tensor x, c10::optional<Tensor> weight,
         check_capture({x, gamma, beta});
         return NormFn::apply(x, maybe(gamma), maybe(beta), eps, act8);
     }
-    return shaped(norm_forward(as_rows(x), contiguous_or_none(gamma),
-                               contiguous_or_none(beta), eps, false, false,
-                               false, false).y.t, x.sizes());
+    return norm_forward(as_rows(x), contiguous_or_none(gamma),
+                        contiguous_or_none(beta), eps, false, false, false,
+                        x.sizes()).y.t;
 }
 
 // ---- linear layer ----------------------------------------------------------------
@@ -224,7 +223,8 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
                              wants_grad(bias);
         LinearOut o = linear_forward(m, wm, contiguous_or_none(bias),
                                      res.defined() ? &r : nullptr, (int)act,
-                                     through, act8, false, false);
+                                     through, act8, false,
+                                     out_sizes(x, w.size(0)));
         Packed x8;
         if (wants_grad(w) && act8) x8 = pack(m);
         // a copy that was made serves the backward pass too
@@ -236,7 +236,7 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
         ctx->saved_data["inputs"] = present({x, w, bias, res});
         ctx->saved_data["act"] = act;
         ctx->saved_data["how"] = (int64_t)o.u.how;
-        return shaped(o.y.t, out_sizes(x, w.size(0)));
+        return o.y.t;
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -259,15 +259,14 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
                                 need_b && !plain ? s[6] : Tensor(), &db, act8);
             if (need_w)
                 dw = weight_grad(p, act8
-                    ? unpack(s[2], s[3], dy.scalar_type(), true)
+                    ? unpack(s[2], s[3], dy.scalar_type(), {})
                     : as_rows(s[0]), plain ? s[6] : Tensor(), &db);
             else if (plain)
                 db = row_sums(p, s[6].scalar_type());
             p.lo = Tensor();
             if (need_x)
-                dx = shaped(input_grad(p, as_rows(s[1]), 0, Kept(), Tensor(),
-                                       nullptr, false).t,
-                            out_sizes(dy, s[1].size(1)));
+                dx = input_grad(p, as_rows(s[1]), 0, Kept(), Tensor(), nullptr,
+                                false, out_sizes(dy, s[1].size(1))).t;
         }
         return {dx, dw, db, needs(ctx, 3) ? dy : Tensor(),
                 Tensor(), Tensor()};
@@ -297,12 +296,11 @@ Tensor linear_act(Tensor x, Tensor weight, c10::optional<Tensor> bias,
     Mat rm;
     const Mat m = as_rows(x);
     if (r.defined()) rm = as_rows(r);
-    return shaped(linear_forward(on_lines(m, weight.size(0)),
-                                 on_lines(as_rows(weight), m.rows),
-                                 contiguous_or_none(b),
-                                 r.defined() ? &rm : nullptr, (int)act, false,
-                                 false, false, false).y.t,
-                  out_sizes(x, weight.size(0)));
+    return linear_forward(on_lines(m, weight.size(0)),
+                          on_lines(as_rows(weight), m.rows),
+                          contiguous_or_none(b), r.defined() ? &rm : nullptr,
+                          (int)act, false, false, false,
+                          out_sizes(x, weight.size(0))).y.t;
 }
 
 // ---- the block ---------------------------------------------------------------------
@@ -317,13 +315,13 @@ struct BlockFn : public torch::autograd::Function<BlockFn> {
         const Mat m = as_rows(x);
         NormOut n = norm_forward(m, contiguous_or_none(gamma),
                                  contiguous_or_none(beta), eps, true, act8,
-                                 act8, true);
+                                 act8, {});
         const Mat r1 = as_rows(w1), r2 = as_rows(w2);
         const Mat m1 = on_lines(r1, m.rows), m2 = on_lines(r2, m.rows);
         LinearOut a = linear_forward(n.y, m1, contiguous_or_none(b1), nullptr,
-                                     (int)act, true, act8, act8, true);
+                                     (int)act, true, act8, act8, {});
         LinearOut o = linear_forward(a.y, m2, contiguous_or_none(b2), &m, 0,
-                                     false, false, false, false);
+                                     false, false, false, x.sizes());
         const Tensor& kept1 = m1.t.is_same(r1.t) ? w1 : m1.t;
         const Tensor& kept2 = m2.t.is_same(r2.t) ? w2 : m2.t;
         const Tensor none;
@@ -335,7 +333,7 @@ struct BlockFn : public torch::autograd::Function<BlockFn> {
         ctx->saved_data["inputs"] = present({x, gamma, beta, w1, b1, w2, b2});
         ctx->saved_data["act"] = act;
         ctx->saved_data["how"] = (int64_t)a.u.how;
-        return shaped(o.y.t, x.sizes());
+        return o.y.t;
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -350,9 +348,9 @@ struct BlockFn : public torch::autograd::Function<BlockFn> {
         auto kept = [&](int plain, int packed) {
             return s[plain].defined()
                 ? as_rows(s[plain])
-                : unpack(s[packed], s[packed + 1], type, true);
+                : unpack(s[packed], s[packed + 1], type, {});
         };
-        Tensor dx, dw1, db1, dw2, db2;
+        Tensor dw1, db1, dw2, db2;
         NormGrads g;
         if (need(5))
             dw2 = weight_grad(d, kept(2, 7), need(6) ? b2 : Tensor(), &db2);
@@ -368,22 +366,21 @@ struct BlockFn : public torch::autograd::Function<BlockFn> {
             const bool act8 = need(3) && !s[1].defined();
             Mat p = input_grad(d, as_rows(w2),
                                (int)ctx->saved_data["act"].toInt(), u,
-                               bias ? b1 : Tensor(), &db1, norm || act8);
+                               bias ? b1 : Tensor(), &db1, norm || act8, {});
             if (norm) {
                 const Mat dh = input_grad(p, as_rows(w1), 0, Kept(), Tensor(),
-                                          nullptr, false);
+                                          nullptr, false, {});
                 g = norm_backward(
                     s[0].defined() ? as_rows(s[0]) : Mat(), {s[3], s[4]},
                     dh, &d, contiguous_or_none(s[12]),
                     contiguous_or_none(s[13]), s[11], need(0),
-                    need(1) || need(2));
-                if (need(0)) dx = shaped(g.dx, dy.sizes());
+                    need(1) || need(2), dy.sizes());
             }
             if (!act8) p.lo = Tensor();
             if (need(3))
                 dw1 = weight_grad(p, kept(1, 5), Tensor(), nullptr);
         }
-        return {dx, g.dgamma, g.dbeta, dw1, db1, dw2, db2, Tensor(), Tensor(),
+        return {g.dx, g.dgamma, g.dbeta, dw1, db1, dw2, db2, Tensor(), Tensor(),
                 Tensor()};
     }
 };
@@ -414,13 +411,13 @@ Tensor ffn_block(Tensor x, c10::optional<Tensor> norm_weight,
     const Mat m = as_rows(x);
     const NormOut n = norm_forward(m, contiguous_or_none(gamma),
                                    contiguous_or_none(beta), eps, false, false,
-                                   false, true);
+                                   false, {});
     const LinearOut a = linear_forward(n.y, on_lines(as_rows(w1), m.rows),
                                        contiguous_or_none(c1), nullptr,
-                                       (int)act, false, false, false, true);
-    return shaped(linear_forward(a.y, on_lines(as_rows(w2), m.rows),
-                                 contiguous_or_none(c2), &m, 0, false, false,
-                                 false, false).y.t, x.sizes());
+                                       (int)act, false, false, false, {});
+    return linear_forward(a.y, on_lines(as_rows(w2), m.rows),
+                          contiguous_or_none(c2), &m, 0, false, false, false,
+                          x.sizes()).y.t;
 }
 
 // ---- the 8-bit form ------------------------------------------------------------------
@@ -428,10 +425,11 @@ std::vector<Tensor> act8_pack(Tensor x) {
     check_seen("act8_pack", {x});
     check_values(x, "x");
     const at::DeviceGuard guard(x.device());
-    const Packed p = pack(as_rows(x));
-    std::vector<int64_t> s = x.sizes().vec();
-    s.back() = p.scales.size(1);
-    return {shaped(p.codes, x.sizes()), shaped(p.scales, s)};
+    const Packed p{at::empty(x.sizes(), x.options().dtype(at::kChar)),
+                   at::empty(out_sizes(x, (x.size(-1) + 127) / 128),
+                             x.options().dtype(at::kFloat))};
+    pack_to(as_rows(x), p);
+    return {p.codes, p.scales};
 }
 
 Tensor act8_unpack(Tensor codes, Tensor scales, int64_t type) {
@@ -457,9 +455,9 @@ Tensor act8_unpack(Tensor codes, Tensor scales, int64_t type) {
     const auto t = type == 0 ? at::kFloat : type == 1 ? at::kBFloat16
                                                       : at::kHalf;
     const int64_t rows = codes.numel() / dim;
-    return shaped(unpack(shaped(codes.contiguous(), {rows, dim}),
-                         shaped(scales.contiguous(), {rows, s.back()}), t,
-                         false).t, codes.sizes());
+    return unpack(shaped(codes.contiguous(), {rows, dim}),
+                  shaped(scales.contiguous(), {rows, s.back()}), t,
+                  codes.sizes()).t;
 }
 
 }  // namespace ffn

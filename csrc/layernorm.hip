@@ -67,8 +67,13 @@ Packed empty_packed(long long rows, long long dim, const at::Tensor& like) {
 
 Packed pack(const Mat& x) {
     Packed p = empty_packed(x.rows, x.dim, x.t);
+    pack_to(x, p);
+    return p;
+}
+
+void pack_to(const Mat& x, const Packed& p) {
     const long long groups = x.rows * groups_in(x.dim);
-    if (!groups) return p;
+    if (!groups) return;
     const int grid = (int)std::min<long long>((groups + 31) / 32, 256 * 64);
     FFN_TYPES(x.t.scalar_type(), FFN_COUNT(groups,
         auto k = act8_pack_kernel<T, I>;
@@ -77,7 +82,16 @@ Packed pack(const Mat& x) {
                            (int)x.dim, (signed char*)p.codes.data_ptr(),
                            p.scales.data_ptr<float>())));
     FFN_OK();
-    return p;
+}
+
+Mat empty_result(at::IntArrayRef sizes, const at::Tensor& like,
+                 at::ScalarType type) {
+    Mat m;
+    m.t = at::empty(sizes, like.options().dtype(type));
+    m.dim = m.ld = sizes.back();
+    m.rows = 1;
+    for (size_t i = 0; i + 1 < sizes.size(); ++i) m.rows *= sizes[i];
+    return m;
 }
 
 Mat empty_rows(long long rows, long long dim, const at::Tensor& like,
@@ -109,16 +123,10 @@ Mat on_lines(const Mat& m, long long other) {
 }
 
 Mat unpack(const at::Tensor& codes, const at::Tensor& scales,
-           at::ScalarType type, bool lines) {
+           at::ScalarType type, at::IntArrayRef sizes) {
     const long long rows = codes.size(0), dim = codes.size(1);
-    Mat out;
-    if (lines) {
-        out = empty_rows(rows, dim, codes, type);
-    } else {
-        out.t = at::empty({rows, dim}, codes.options().dtype(type));
-        out.rows = rows;
-        out.dim = out.ld = dim;
-    }
+    const Mat out = sizes.empty() ? empty_rows(rows, dim, codes, type)
+                                  : empty_result(sizes, codes, type);
     const long long n = rows * ((dim + 7) / 8);
     if (!n) return out;
     const int grid = (int)std::min<long long>((n + 255) / 256, 1 << 22);
@@ -168,15 +176,11 @@ Mat unpack(const at::Tensor& codes, const at::Tensor& scales,
 
 NormOut norm_forward(const Mat& x, const at::Tensor& gamma,
                      const at::Tensor& beta, double eps, bool stats,
-                     bool keep_x8, bool keep_y8, bool lines) {
+                     bool keep_x8, bool keep_y8, at::IntArrayRef sizes) {
     NormOut o;
-    if (lines) {
-        o.y = empty_rows(x.rows, x.dim, x.t, x.t.scalar_type());
-    } else {
-        o.y.t = at::empty({x.rows, x.dim}, x.t.options());
-        o.y.rows = x.rows;
-        o.y.dim = o.y.ld = x.dim;
-    }
+    const auto type = x.t.scalar_type();
+    o.y = sizes.empty() ? empty_rows(x.rows, x.dim, x.t, type)
+                        : empty_result(sizes, x.t, type);
     if (stats)
         o.stats = at::empty({2, x.rows}, x.t.options().dtype(at::kFloat));
     if (keep_x8) o.x8 = empty_packed(x.rows, x.dim, x.t);
@@ -218,7 +222,7 @@ NormOut norm_forward(const Mat& x, const at::Tensor& gamma,
         auto k = norm_forward_wide_kernel<T>; \
         hipLaunchKernelGGL(k, (int)x.rows, 1024, 0, s, a); \
     } while (0)
-    FFN_TYPES(x.t.scalar_type(), NORM_SHAPES(x.dim, WIDE, GO));
+    FFN_TYPES(type, NORM_SHAPES(x.dim, WIDE, GO));
     #undef GO
     #undef WIDE
     FFN_OK();
@@ -240,10 +244,11 @@ static void sum_columns(const at::Tensor& part, long long n, long long width,
 NormGrads norm_backward(const Mat& x, const Packed& x8, const Mat& dy,
                         const Mat* add, const at::Tensor& gamma,
                         const at::Tensor& beta, const at::Tensor& stats,
-                        bool need_dx, bool need_params) {
+                        bool need_dx, bool need_params,
+                        at::IntArrayRef sizes) {
     const long long rows = dy.rows, dim = dy.dim;
     NormGrads g;
-    if (need_dx) g.dx = at::empty({rows, dim}, dy.t.options());
+    if (need_dx) g.dx = at::empty(sizes, dy.t.options());
     if (need_params && gamma.defined()) g.dgamma = at::empty_like(gamma);
     if (need_params && beta.defined()) g.dbeta = at::empty_like(beta);
     const bool params = g.dgamma.defined() || g.dbeta.defined();

@@ -188,16 +188,11 @@ static void set_kept(EpiArgs& e, const Kept& u) {
 
 LinearOut linear_forward(const Mat& x, const Mat& w, const at::Tensor& bias,
                          const Mat* res, int act, bool keep, bool act8,
-                         bool keep_y8, bool lines) {
+                         bool keep_y8, at::IntArrayRef sizes) {
     LinearOut o;
     const long long M = x.rows, N = w.rows;
-    if (lines) {
-        o.y = empty_rows(M, N, x.t, x.t.scalar_type());
-    } else {
-        o.y.t = at::empty({M, N}, x.t.options());
-        o.y.rows = M;
-        o.y.dim = o.y.ld = N;
-    }
+    o.y = sizes.empty() ? empty_rows(M, N, x.t, x.t.scalar_type())
+                        : empty_result(sizes, x.t, x.t.scalar_type());
     if (keep) o.u = empty_kept(act, act8, M, N, x.t);
     if (keep_y8) o.y8 = empty_packed(M, N, x.t);
     if (!M) return o;
@@ -291,16 +286,14 @@ Mat through_act(const Mat& dy, int act, const Kept& u, const at::Tensor& bias,
 }
 
 Mat input_grad(const Mat& p, const Mat& w, int act, const Kept& u,
-               const at::Tensor& bias, at::Tensor* dbias, bool split) {
+               const at::Tensor& bias, at::Tensor* dbias, bool split,
+               at::IntArrayRef sizes) {
     const long long M = p.rows, N = w.dim;
-    Mat out;
-    if (act != ACT_NONE) {      // goes on into products
-        out = empty_grad(M, N, p.t, split, u);
-    } else {
-        out.t = at::empty({M, N}, p.t.options());
-        out.rows = M;
-        out.dim = out.ld = N;
-    }
+    const auto type = p.t.scalar_type();
+    const int64_t plain[] = {M, N};
+    const Mat out =
+        act != ACT_NONE ? empty_grad(M, N, p.t, split, u) // goes into products
+                        : empty_result(sizes.empty() ? plain : sizes, p.t, type);
     if (!M) {
         if (bias.defined()) *dbias = at::zeros_like(bias);
         return out;
@@ -314,8 +307,8 @@ Mat input_grad(const Mat& p, const Mat& w, int act, const Kept& u,
     Colsum sum;
     if (bias.defined()) sum.aim(e, M, N, bias, M <= 16);
     long long blocks;
-    product<true, false, EPI_GRAD>(p.t.scalar_type(), operand(p), operand(w),
-                                   M, N, p.dim, e, p.t, &blocks);
+    product<true, false, EPI_GRAD>(type, operand(p), operand(w), M, N, p.dim,
+                                   e, p.t, &blocks);
     if (bias.defined()) *dbias = sum.join(blocks);
     return out;
 }
