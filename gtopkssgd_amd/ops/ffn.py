@@ -15,10 +15,12 @@ from typing import Optional
 
 import torch
 import torch.nn as nn
+import torch.nn.functional as F
+from torch.nn.modules import module as _module
 
 from . import _ext
 from .layernorm import FusedLayerNorm, layer_norm
-from .linear import _act_code, linear_act
+from .linear import FusedLinearAct, _act_code, linear_act
 
 
 def ffn_block(x: torch.Tensor, norm_weight: Optional[torch.Tensor],
@@ -51,20 +53,47 @@ def ffn_block(x: torch.Tensor, norm_weight: Optional[torch.Tensor],
     return linear_act(a, w2, b2, residual=x, act8=act8)
 
 
+def _nothing_hangs_on(m: nn.Module) -> bool:
+    """Calling ``m`` does what its parameters say, and nothing else."""
+    return not (m._forward_pre_hooks or m._forward_hooks or
+                m._backward_pre_hooks or m._backward_hooks or
+                "forward" in vars(m))
+
+
 class FFNBlock(nn.Module):
-    """``ffn_block`` with its parameters."""
+    """``ffn_block`` with its parameters.
+
+    Its children ``norm``, ``fc1`` and ``fc2`` are the layer norm and the two
+    linear layers without activation or residual, and keep the parameters.  They
+    are called, with the activation and the addition of x between and after
+    them, where something hangs on that: hooks of theirs or of all modules
+    (pruning and the like work by such), or another module in a child's place.
+    Otherwise the block is one call, with fewer roundings on its way."""
 
     def __init__(self, dim: int, hidden: int, act: str = "gelu",
                  act8: bool = False, eps: float = 1e-5):
         super().__init__()
         _act_code(act)
         self.norm = FusedLayerNorm(dim, eps=eps, act8=act8)
-        self.fc1 = nn.Linear(dim, hidden)
-        self.fc2 = nn.Linear(hidden, dim)
+        self.fc1 = FusedLinearAct(dim, hidden, act8=act8)
+        self.fc2 = FusedLinearAct(hidden, dim, act8=act8)
         self.act = act
         self.act8 = act8
 
+    def _as_one_call(self) -> bool:
+        fc = (self.fc1, self.fc2)
+        return type(self.norm) is FusedLayerNorm and \
+            all(type(m) is FusedLinearAct and m.act == "none" for m in fc) and \
+            all(map(_nothing_hangs_on, (self.norm, *fc))) and \
+            not _module._has_any_global_hook()
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if not self._as_one_call():
+            if x.is_cuda and torch.is_autocast_enabled("cuda"):
+                x = x.to(torch.get_autocast_dtype("cuda"))
+            u = self.fc1(self.norm(x))
+            a = u if self.act == "none" else getattr(F, self.act)(u)
+            return x + self.fc2(a)
         return ffn_block(x, self.norm.weight, self.norm.bias, self.fc1.weight,
                          self.fc1.bias, self.fc2.weight, self.fc2.bias,
                          self.act, self.norm.eps, self.act8)
