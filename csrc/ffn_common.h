@@ -233,24 +233,29 @@ __device__ __forceinline__ float wave_sum(float v) {
 }
 
 // ---- activations -----------------------------------------------------------
-// q = Phi(-|u|), the normal distribution's tail, and e = exp(-u^2 / 2).  FAST:
-// Abramowitz & Stegun 7.1.26, erf(z) = 1 - t P(t) exp(-z^2) with t = 1 / (1 + p z)
-// and z = |u| / sqrt(2), |error| < 1.5e-7: under 2^-22, while the 16-bit types
-// that it serves round to 2^-12 at best.  One exp and one reciprocal; the
-// epilogues that use it are bound by the vector unit.  Otherwise erfcf.
+// q = Phi(-|u|), the normal distribution's tail, and e = exp(-u^2 / 2).  Below 0
+// gelu is u q, and its slope q + u phi: q has to be right relative to itself,
+// as far down as the types hold it.  FAST, for 16 bits: q = e t P(t), t = 1 / (1
+// + p |u|), the form of Abramowitz & Stegun 7.1.26, with p and the 6 coefficients
+// of P fitted over 0..14 for the least relative error of q, which may be min(1 /
+// (2 q), 32) times as large as at 0: 2^-21 there, 2^-16 in the tail.  In fp32
+// arithmetic under 2^-21 absolute, and 2^-15.7 of q down to u = -13; 16-bit types
+// round by 2^-11 at best.  (Fitted for the absolute error, as published, it is off
+// by 2^-11 of q at u = -4 and 2^-6 at -9.)  One exp and one reciprocal; the epilogues
+// that use it are bound by the vector unit.  Otherwise erfcf.
 template <bool FAST>
 __device__ __forceinline__ float normal_tail(float u, float* e) {
     const float z = fabsf(u);
     if (FAST) {
         // exp2(-u^2 / 2 * log2(e))
         *e = __builtin_amdgcn_exp2f(u * (u * -0.72134752044f));
-        // p / sqrt(2); the coefficients are halved
         const float t = __builtin_amdgcn_rcpf(
-            __builtin_fmaf(z, 0.23164189f, 1.0f));
-        float q = __builtin_fmaf(t, 0.5307027145f, -0.7265760135f);
-        q = __builtin_fmaf(t, q, 0.7107068705f);
-        q = __builtin_fmaf(t, q, -0.142248368f);
-        q = __builtin_fmaf(t, q, 0.127414796f);
+            __builtin_fmaf(z, 0.29928696f, 1.0f));
+        float q = __builtin_fmaf(t, -0.08004875f, 0.22636297f);
+        q = __builtin_fmaf(t, q, -0.027499145f);
+        q = __builtin_fmaf(t, q, 0.14891709f);
+        q = __builtin_fmaf(t, q, 0.11239303f);
+        q = __builtin_fmaf(t, q, 0.11987457f);
         return q * t * *e;
     }
     *e = expf(-0.5f * u * u);
@@ -282,7 +287,7 @@ __device__ __forceinline__ float act_slope(float u, int act) {
         // Phi(u) + u phi(u), phi(u) = e / sqrt(2 pi); a NaN is in cdf
         float e;
         const float q = normal_tail<FAST>(u, &e);
-        const float cdf = 0.5f + __builtin_copysignf(0.5f - q, u);
+        const float cdf = u < 0.0f ? q : 1.0f - q;
         return __builtin_fmaf(__builtin_amdgcn_fmed3f(u, -16.0f, 16.0f) * e,
                               0.3989422804014327f, cdf);
     }
