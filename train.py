@@ -80,6 +80,16 @@ def parse_args():
     return args
 
 
+def default_run_tag(args, world):
+    """The name under which a run's checkpoints lie: what tells its model from
+    another is part of it."""
+    tag = (f"{args.dnn}-{args.dataset}-bs{args.batch_size}-"
+           f"rho{args.density}-{args.compression}-n{world}")
+    if args.ffn_mult:
+        tag += f"-ffn{args.ffn_mult}" + ("-act8" if args.act8 else "")
+    return tag
+
+
 def init_dist(args):
     if "WORLD_SIZE" in os.environ and int(os.environ["WORLD_SIZE"]) > 1:
         use_gpu = torch.cuda.is_available() and args.device != "cpu"
@@ -99,9 +109,7 @@ def init_dist(args):
 def main():
     args = parse_args()
     rank, world = init_dist(args)
-    run_tag = args.run_tag or (
-        f"{args.dnn}-{args.dataset}-bs{args.batch_size}-"
-        f"rho{args.density}-{args.compression}-n{world}")
+    run_tag = args.run_tag or default_run_tag(args, world)
     metrics = JsonlLogger(args.metrics) if args.metrics and rank == 0 else None
 
     model_kwargs = {"ffn_mult": args.ffn_mult, "act8": args.act8} \
