@@ -99,7 +99,7 @@ static bool recording(std::initializer_list<Tensor> all) {
 // A leaf's gradient goes to it on the stream on which its first graph that still
 // lives was recorded.  Captured, that would be work on a stream that is not part
 // of the capture, which the autograd engine's thread does not survive.
-static void check_capture(std::initializer_list<Tensor> all) {
+static void check_capture(at::ArrayRef<Tensor> all) {
     const auto stream = c10::hip::getCurrentHIPStream();
     hipStreamCaptureStatus status;
     if (hipStreamIsCapturing(stream, &status) == hipSuccess &&
@@ -115,6 +115,13 @@ static void check_capture(std::initializer_list<Tensor> all) {
                     "input of this captured call: free that graph (its outputs)"
                     " before the capture begins");
     }
+}
+
+// the same for leaves that the caller casts before it passes them on
+void check_cast_leaves(const std::vector<Tensor>& all) {
+    if (!at::GradMode::is_enabled() || all.empty() || !all[0].is_cuda()) return;
+    const at::DeviceGuard guard(all[0].device());
+    check_capture(all);
 }
 
 static void check_once(const char* name) {

@@ -88,6 +88,7 @@ at::Tensor ffn_block(at::Tensor x, c10::optional<at::Tensor> norm_weight,
                      c10::optional<at::Tensor> b1, at::Tensor w2,
                      c10::optional<at::Tensor> b2, int64_t act, double eps,
                      bool act8);
+void check_cast_leaves(const std::vector<at::Tensor>& all);
 std::vector<at::Tensor> act8_pack(at::Tensor x);
 at::Tensor act8_unpack(at::Tensor codes, at::Tensor scales, int64_t type);
 

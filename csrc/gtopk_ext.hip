@@ -750,6 +750,7 @@ at::Tensor ffn_block(at::Tensor x, c10::optional<at::Tensor> norm_weight,
                      c10::optional<at::Tensor> b1, at::Tensor w2,
                      c10::optional<at::Tensor> b2, int64_t act, double eps,
                      bool act8);
+void check_cast_leaves(const std::vector<at::Tensor>& all);
 std::vector<at::Tensor> act8_pack(at::Tensor x);
 at::Tensor act8_unpack(at::Tensor codes, at::Tensor scales, int64_t type);
 }  // namespace ffn
@@ -761,6 +762,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           "act(x W^T + b) + residual with its backward pass (gfx950)");
     m.def("ffn_block", &ffn::ffn_block,
           "x + W2 act(W1 norm(x) + b1) + b2 with its backward pass (gfx950)");
+    m.def("check_cast_leaves", &ffn::check_cast_leaves,
+          "refuses a captured call whose leaves a living eager graph keeps");
     m.def("act8_pack", &ffn::act8_pack, "8-bit form of an activation");
     m.def("act8_unpack", &ffn::act8_unpack, "values of an 8-bit form");
     m.def("bn_fwd_train", &bn_fwd_train,

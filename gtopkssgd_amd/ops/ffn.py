@@ -19,6 +19,7 @@ import torch.nn.functional as F
 from torch.nn.modules import module as _module
 
 from . import _ext
+from ._autocast import check_cast_leaves
 from .layernorm import FusedLayerNorm, layer_norm
 from .linear import FusedLinearAct, _act_code, linear_act
 
@@ -38,6 +39,7 @@ def ffn_block(x: torch.Tensor, norm_weight: Optional[torch.Tensor],
     code = _act_code(act)
     if x.is_cuda:
         if torch.is_autocast_enabled("cuda"):
+            check_cast_leaves(x, norm_weight, norm_bias, w1, b1, w2, b2)
             t = torch.get_autocast_dtype("cuda")
             x, w1, w2 = x.to(t), w1.to(t), w2.to(t)
             norm_weight, norm_bias, b1, b2 = (
@@ -90,6 +92,7 @@ class FFNBlock(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if not self._as_one_call():
             if x.is_cuda and torch.is_autocast_enabled("cuda"):
+                check_cast_leaves(x)
                 x = x.to(torch.get_autocast_dtype("cuda"))
             u = self.fc1(self.norm(x))
             a = u if self.act == "none" else getattr(F, self.act)(u)

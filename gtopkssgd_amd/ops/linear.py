@@ -20,6 +20,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import _ext
+from ._autocast import check_cast_leaves
 from .act8 import _wide, act8_pack, act8_unpack
 
 ACTS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
@@ -105,6 +106,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor,
     code = _act_code(act)
     if x.is_cuda:
         if torch.is_autocast_enabled("cuda"):
+            check_cast_leaves(x, weight, bias, residual)
             t = torch.get_autocast_dtype("cuda")
             x, weight = x.to(t), weight.to(t)
             residual = None if residual is None else residual.to(t)
