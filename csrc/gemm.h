@@ -42,7 +42,8 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 // 64 lanes x 16 bytes from memory straight into LDS at `lds` + PLUS + 16 * lane.
 // Offsets (both parts of it) at or past the descriptor's size read as zeros.
 // Nothing here tells the compiler that the bytes are on their way: stage_wait()
-// does, for all.  m0 is set anew by each copy and used by nothing else.
+// does, for all.  m0 is set anew by each copy; it is reserved, cannot be named as
+// clobbered, and the compiler's own code for these kernels does not touch it.
 template <int PLUS>
 __device__ __forceinline__ void dma16(u32x4 desc, unsigned lds, int voff,
                                       unsigned soff) {
