@@ -75,6 +75,8 @@ Mat input_grad(const Mat& p, const Mat& w, int act, const Kept& u,
 at::Tensor weight_grad(const Mat& p, const Mat& x, const at::Tensor& bias,
                        at::Tensor* dbias);
 at::Tensor row_sums(const Mat& p, at::ScalarType type);
+// out = sum of the first n rows of partial sums
+void sum_partials(const at::Tensor& part, long long n, at::Tensor& out);
 
 // autograd entry points, bound in gtopk_ext.hip
 at::Tensor layer_norm(at::Tensor x, c10::optional<at::Tensor> weight,

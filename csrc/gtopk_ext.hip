@@ -20,6 +20,7 @@
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <hip/hip_runtime.h>
+#include "ffn_ops.h"
 
 #define HIST_BITS 13
 #define HIST_BINS (1 << HIST_BITS)   // 8192
@@ -736,24 +737,6 @@ std::vector<at::Tensor> bn_bwd(
     at::Tensor dy, at::Tensor x, c10::optional<at::Tensor> y,
     at::Tensor gamma, at::Tensor saved_mean, at::Tensor saved_rstd,
     bool relu, bool need_dz, at::Tensor stats_scratch);
-
-// feed-forward operators (ffn_autograd.hip)
-namespace ffn {
-at::Tensor layer_norm(at::Tensor x, c10::optional<at::Tensor> weight,
-                      c10::optional<at::Tensor> bias, double eps, bool act8);
-at::Tensor linear_act(at::Tensor x, at::Tensor weight,
-                      c10::optional<at::Tensor> bias,
-                      c10::optional<at::Tensor> residual, int64_t act,
-                      bool act8);
-at::Tensor ffn_block(at::Tensor x, c10::optional<at::Tensor> norm_weight,
-                     c10::optional<at::Tensor> norm_bias, at::Tensor w1,
-                     c10::optional<at::Tensor> b1, at::Tensor w2,
-                     c10::optional<at::Tensor> b2, int64_t act, double eps,
-                     bool act8);
-void check_cast_leaves(const std::vector<at::Tensor>& all);
-std::vector<at::Tensor> act8_pack(at::Tensor x);
-at::Tensor act8_unpack(at::Tensor codes, at::Tensor scales, int64_t type);
-}  // namespace ffn
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("layer_norm", &ffn::layer_norm,

@@ -1,26 +1,10 @@
 // Layer norm forward and backward, the 8-bit form of activations, and sums
 // over rows: launches.
 #include <hip/hip_runtime.h>
-#include "ffn_ops.h"
-#include <c10/hip/HIPStream.h>
+#include "ffn_launch.h"
 #include "layernorm_kernels.h"
 
 namespace ffn {
-
-#define FFN_OK() do { hipError_t _e = hipGetLastError(); \
-    TORCH_CHECK(_e == hipSuccess, "HIP error: ", hipGetErrorString(_e)); \
-} while (0)
-
-// runs the statement with T as the tensor's type
-#define FFN_TYPES(type, ...) do { \
-    if ((type) == at::kBFloat16) { typedef bf16_t T; __VA_ARGS__; } \
-    else if ((type) == at::kHalf) { typedef f16_t T; __VA_ARGS__; } \
-    else { typedef float T; __VA_ARGS__; } \
-} while (0)
-
-static hipStream_t stream_now() {
-    return c10::hip::getCurrentHIPStream().stream();
-}
 
 Mat as_rows(const at::Tensor& x) {
     Mat m;
@@ -341,7 +325,6 @@ at::Tensor row_sums(const Mat& p, at::ScalarType type) {
     return out;
 }
 
-// out = sum of the first n rows of partial sums, for linear.hip
 void sum_partials(const at::Tensor& part, long long n, at::Tensor& out) {
     sum_columns(part, n, out.numel(), out.numel(), out, at::Tensor());
 }

@@ -1,26 +1,9 @@
 // Products of linear layers: choice of tile and of the split over k, launches.
 #include <hip/hip_runtime.h>
-#include "ffn_ops.h"
-#include <c10/hip/HIPStream.h>
+#include "ffn_launch.h"
 #include "linear_kernels.h"
 
 namespace ffn {
-
-#define FFN_OK() do { hipError_t _e = hipGetLastError(); \
-    TORCH_CHECK(_e == hipSuccess, "HIP error: ", hipGetErrorString(_e)); \
-} while (0)
-
-#define FFN_TYPES(type, ...) do { \
-    if ((type) == at::kBFloat16) { typedef bf16_t T; __VA_ARGS__; } \
-    else if ((type) == at::kHalf) { typedef f16_t T; __VA_ARGS__; } \
-    else { typedef float T; __VA_ARGS__; } \
-} while (0)
-
-void sum_partials(const at::Tensor& part, long long n, at::Tensor& out);
-
-static hipStream_t stream_now() {
-    return c10::hip::getCurrentHIPStream().stream();
-}
 
 // up to this many rows of an operand along k go to thin_kernel
 #define THIN_ROWS 64
