@@ -5,7 +5,11 @@
 #include "gemm.h"
 
 enum Epilogue { EPI_FORWARD = 0, EPI_GRAD = 1, EPI_PLAIN = 2 };
-// how the value before the activation is kept for the backward pass
+// How the value before the activation, u, is kept for the backward pass.  In full
+// means in the type: a u of 32 bits would double what is written and read, and
+// what its rounding does to the slope is small beside p's own (db, summed before
+// p rounds: 0.00175 of its norm off in bf16, where the last rounding makes
+// 0.0017).
 enum Keep { KEEP_NONE = 0, KEEP_FULL = 1, KEEP_BITS = 2, KEEP_8BIT = 3 };
 
 struct EpiArgs {
