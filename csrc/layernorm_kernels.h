@@ -83,7 +83,10 @@ __device__ __forceinline__ float norm_rstd(float q, float more, float n,
 // chunks of 8 a thread: x is read once, the mean comes first and the variance
 // from what is left of it.  Bound by memory: 32768 x 2048 in fp32 99 us (5.4
 // TB/s), and nearly so by instructions in 16 bits with the 8-bit form: 17920 x
-// 1500 32 us (4.2 TB/s).
+// 1500 32 us (4.2 TB/s).  Four chunks for each of 1024 threads, rows of 16385 to
+// 32768 values, do not fit their 128 registers: 68 (16 bits) or 300 bytes a lane
+// go to scratch memory, and 32768 values go at 2.8 and 2.1 TB/s where 8192 go at
+// 5.3.
 template <typename T, int NT, int R>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void norm_forward_kernel(
         NormArgs p) {
@@ -237,7 +240,12 @@ __device__ __forceinline__ void load_kept(const NormGradArgs& p, long long row,
 // each thread sums dy xh and dy for its own columns over the rows that it
 // sees, the teams of a block add theirs in turn, and column_sum_kernel adds
 // the blocks': no atomics, the same result each time.  32768 x 2048 in fp32 151
-// us (5.3 TB/s).
+// us (5.3 TB/s).  Two and four chunks a thread, rows of 8193 to 32768 values, do
+// not fit the 128 registers that 1024 threads leave each: 112 to 276 and 824 to
+// 860 bytes a lane go to scratch memory.  Forward and backward, TB/s of x twice,
+// dy, y and dx, in bf16 and fp32: 8192 values 4.9 and 5.2; 9216 2.2 and 2.6, a
+// second chunk that is nearly empty; 16384 3.0 and 3.7; 32768 0.8 and 1.6; 40960,
+// by the kernels for longer rows, 2.7 and 2.6.
 template <typename T, int NT, int R, bool X8>
 __global__ __launch_bounds__(NT < 128 ? 256 : NT) void norm_backward_kernel(
         NormGradArgs p) {

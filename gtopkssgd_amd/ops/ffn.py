@@ -34,8 +34,10 @@ def ffn_block(x: torch.Tensor, norm_weight: Optional[torch.Tensor],
     x: [..., dim], w1: [hidden, dim], w2: [dim, hidden], of one type (bf16,
     fp16 or fp32); norm_weight, norm_bias: [dim], b1: [hidden], b2: [dim], of
     that type or fp32, or None.  Under autocast x, w1 and w2 are cast to its
-    type.  No second derivative; on the GPU forward mode, torch.func's
-    transforms and tracing are refused."""
+    type, and with x the residual: y has that type, too, as a linear layer's
+    result; a residual of fp32 needs the block in fp32, outside autocast.  No
+    second derivative; on the GPU forward mode, torch.func's transforms and
+    tracing are refused."""
     code = _act_code(act)
     if x.is_cuda:
         if torch.is_autocast_enabled("cuda"):
