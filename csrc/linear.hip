@@ -158,7 +158,10 @@ static Kept empty_kept(int act, bool act8, long long rows, long long dim,
         u.scales = p.scales;
     } else if (act != ACT_NONE) {
         u.how = KEEP_FULL;
-        u.data = at::empty({rows, dim}, like.options());
+        // KeptType
+        const auto t = like.scalar_type() == at::kBFloat16 ? at::kHalf
+                                                           : at::kFloat;
+        u.data = at::empty({rows, dim}, like.options().dtype(t));
     }
     return u;
 }

@@ -5,12 +5,19 @@
 #include "gemm.h"
 
 enum Epilogue { EPI_FORWARD = 0, EPI_GRAD = 1, EPI_PLAIN = 2 };
-// How the value before the activation, u, is kept for the backward pass.  In full
-// means in the type: a u of 32 bits would double what is written and read, and
-// what its rounding does to the slope is small beside p's own (db, summed before
-// p rounds: 0.00175 of its norm off in bf16, where the last rounding makes
-// 0.0017).
+// how the value before the activation, u, is kept for the backward pass
 enum Keep { KEEP_NONE = 0, KEEP_FULL = 1, KEEP_BITS = 2, KEEP_8BIT = 3 };
+
+// What a u in full is kept as, where the results are T: with more bits than they.
+// Its rounding goes into the slope and from there into each p, and the sums that
+// follow a rounding of their own, the norm's gradients in the block, show it: kept
+// in T, the norm bias's gradient was off by 1.8 times what its rounding makes, so by
+// 1.1.  bf16: fp16 has 3 bits more in the same place, and where it ends, at 65504
+// and 2^-24, a slope is 0, 1 or 1/2 already; a linear layer of 17920 x 1500 to 6000
+// with gelu, forward and backward, takes 1265 us for 1267.  fp16: twice the bytes,
+// there 215 MB more and 1359 us for 1291, at 700 rows 119 for 116.
+template <typename T> struct KeptType { typedef float V; };
+template <> struct KeptType<bf16_t> { typedef f16_t V; };
 
 struct EpiArgs {
     void* out;             // [M, N] of T
@@ -19,7 +26,7 @@ struct EpiArgs {
     const void* bias;      // [N] of T (of float where bias_f32) or null
     const void* res;       // [M, N] of T or null
     long long ld_res;
-    void* kept;            // [M, N] of T, [M, N / 8] bytes, or [M, N] codes
+    void* kept;            // [M, N] of KeptType, [M, N / 8] bytes, or codes
     float* kept_scale;     // [M, N / 128]
     signed char* out8;     // 8-bit form of `out`, or null
     float* out8_scale;
@@ -38,6 +45,7 @@ template <> struct IsHalf<float> { static constexpr bool value = false; };
 // kept of the value before the activation.  It is fetched long before its use.
 template <typename T> struct Extra {
     typename Chunk<T>::V v;
+    typename Chunk<typename KeptType<T>::V>::V u;
     u32x2 codes;
     float scale;
     unsigned bits;
@@ -57,7 +65,7 @@ __device__ __forceinline__ void fetch_extra(Extra<T>& x, const EpiArgs& e,
         if (e.res) x.v = fetch8((const T*)e.res + m * e.ld_res, n, N);
     } else if (EPI == EPI_GRAD) {
         if (e.keep == KEEP_FULL) {
-            x.v = fetch8((const T*)e.kept + m * N, n, N);
+            x.u = fetch8((const typename KeptType<T>::V*)e.kept + m * N, n, N);
         } else if (e.keep == KEEP_8BIT) {
             const signed char* p = (const signed char*)e.kept + m * N;
             if (N >= 8) {
@@ -122,7 +130,7 @@ __device__ __forceinline__ void finish8(float* v, long long m, int n, int left,
                 #pragma unroll
                 for (int i = 0; i < 8; ++i) u[i] *= x.scale;
             } else {
-                unpack8(x.v, n, N, whole, u);
+                unpack8(x.u, n, N, whole, u);
             }
             #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] *= act_slope<FAST>(u[i], e.act);
@@ -155,7 +163,8 @@ __device__ __forceinline__ void finish8(float* v, long long m, int n, int left,
             ((unsigned char*)e.kept)[m * ((N + 7) >> 3) + (n >> 3)] =
                 (unsigned char)bits;
     } else if (e.keep == KEEP_FULL) {
-        if (on) store8((T*)e.kept + m * N + n, left, v);
+        if (on)
+            store8((typename KeptType<T>::V*)e.kept + m * N + n, left, v);
     } else if (e.keep == KEEP_8BIT) {
         const Act8Scale s = act8_scale(max16(max8(v)));
         if (on) {

@@ -5,7 +5,8 @@ and its backward pass (csrc/linear.hip).
     p = dy act'(u),  u = x W^T + b
     dx = p W,  dW = p^T x,  db = sum of p over the rows,  dresidual = dy
 
-For the backward pass the layer keeps x, W and, for gelu and silu, u; relu
+For the backward pass the layer keeps x, W and, for gelu and silu, u (on the GPU
+with more bits than the result: in fp16 beside bf16, in fp32 beside fp16); relu
 keeps one bit a value.  ``act8=True`` keeps x and u in 8 bits (``act8``
 module): half the memory, and gradients from what those stand for.  On the GPU
 long 16-bit operands of wide products are copied to rows that start on lines of

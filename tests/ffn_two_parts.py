@@ -28,6 +28,13 @@ def summed(a, b, da, parts):
     return a @ b, (terms + 8) * E * (a.abs() @ b.abs()) + da @ b.abs()
 
 
+def rounded_to(v, off, t):
+    """v, off by `off`, rounded: to one value, but for those within their error
+    of a border"""
+    low, high = (v - off).to(t).double(), (v + off).to(t).double()
+    return (low + high) / 2, (high - low) / 2
+
+
 def normal(*shape, t=FP, seed=0, scale=1.0, shift=0.0):
     g = torch.Generator().manual_seed(seed + sum(shape))
     return (torch.randn(*shape, generator=g) * scale + shift).to(t)
@@ -81,17 +88,19 @@ def block_inputs(rows, d, h, t):
             normal(d, h, t=t, scale=h ** -0.5, seed=5), normal(d, t=t, seed=6)]
 
 
-def norm_grads(x, nw, w1, u, da, dy, act, lo=True):
-    """[dx, dweight, dbias] of the norm, and dy onto dx, from the kept u and the
-    rounded da."""
+def norm_grads(x, nw, w1, b1, hid, da, dy, act, lo=True):
+    """[dx, dweight, dbias] of the norm, and dy onto dx, from the rounded hid and
+    da."""
     t = x.dtype
-    x, nw, w1, u, da, dy = map(ref.wide, (x, nw, w1, u, da, dy))
+    x, nw, w1, b1, hid, da, dy = map(ref.wide, (x, nw, w1, b1, hid, da, dy))
+    u, du = summed(hid, w1.t(), torch.zeros_like(hid), 1)
+    u = u + b1
+    u, du = rounded_to(u, du + 2 * E * b1.abs(), HF if t == BF else FP)
     whole, dp = p_of(da, u, act, t, True)
+    dp = dp + ref.CURVE * du * da.abs()
     p = whole if lo else p_of(da, u, act, t, False)[0]
     v, bound = summed(whole, w1, dp, 2)
-    # dh rounds: to one value, but for those within their error of a border
-    low, high = (v - bound).to(t).double(), (v + bound).to(t).double()
-    dh, ddh = (low + high) / 2, (high - low) / 2
+    dh, ddh = rounded_to(v, bound, t)
     if not lo:
         dh = (p @ w1).to(t).double()
     dx, dw, db = ref.norm(x, nw, None, 1e-5, t, dy=dh)[1:]

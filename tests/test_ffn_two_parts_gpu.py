@@ -36,16 +36,15 @@ def test_norm_gradients_of_the_block(t, act, rows, d, h):
     the same bits."""
     args = [v.to(DEV).requires_grad_(True)
             for v in parts.block_inputs(rows, d, h, t)]
-    dy = parts.normal(rows, d, t=t, seed=9, scale=0.01).to(DEV)
+    dy = parts.normal(rows, d, t=t, seed=9, scale=0.25).to(DEV)
     x, nw, nb, w1, b1, w2, b2 = args
     with torch.no_grad():
         hid = gt.layer_norm(x, nw, nb)
-        u = gt.linear_act(hid, w1, b1)
         a = gt.linear_act(hid, w1, b1, act=act)
     a.requires_grad_(True)
     da, = torch.autograd.grad(gt.linear_act(a, w2, b2, x), a, dy)
     got = torch.autograd.grad(gt.ffn_block(*args, act=act), [x, nw, nb], dy)
-    want = parts.norm_grads(x, nw, w1, u, da, dy, act)
+    want = parts.norm_grads(x, nw, w1, b1, hid, da, dy, act)
     ref.close(got[2], *want[2], what="norm bias")
     ref.close(got[1], *want[1], what="norm weight")
     ref.close(got[0], *ref.rounded(*want[0], t), what="dx")
