@@ -379,13 +379,14 @@ struct BlockFn : public torch::autograd::Function<BlockFn> {
             const Kept u{s[9], s[10], (int)ctx->saved_data["how"].toInt()};
             // The norm's gradients are sums over dh, which is rounded as it
             // comes from the product: were p rounded before, dh would round
-            // to other values.  The weight's gradient: as in LinearFn (from
-            // both parts, without 8 bits, the block takes 268 us for 254 at
-            // 700 x 1500, hidden 6000).
-            const bool act8 = need(3) && !s[1].defined();
+            // to other values.  Both parts go into dW1, too: 268 us for 254 at
+            // 700 x 1500, hidden 6000, where LinearFn's two products would take
+            // half as long again; dW1 is off by what its own rounding makes,
+            // not 1.4 times that.
             Mat p = input_grad(d, as_rows(w2),
                                (int)ctx->saved_data["act"].toInt(), u,
-                               bias ? b1 : Tensor(), &db1, norm || act8, {});
+                               bias ? b1 : Tensor(), &db1, norm || need(3),
+                               {});
             if (norm) {
                 const Mat dh = input_grad(p, as_rows(w1), 0, Kept(), Tensor(),
                                           nullptr, false, {});
@@ -395,7 +396,6 @@ struct BlockFn : public torch::autograd::Function<BlockFn> {
                     contiguous_or_none(s[13]), s[11], need(0),
                     need(1) || need(2), dy.sizes());
             }
-            if (!act8) p.lo = Tensor();
             if (need(3))
                 dw1 = weight_grad(p, kept(1, 5), Tensor(), nullptr);
         }

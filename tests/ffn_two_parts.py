@@ -89,8 +89,8 @@ def block_inputs(rows, d, h, t):
 
 
 def norm_grads(x, nw, w1, b1, hid, da, dy, act, lo=True):
-    """[dx, dweight, dbias] of the norm, and dy onto dx, from the rounded hid and
-    da."""
+    """[dx, dweight, dbias] of the norm, dy onto dx, and dw1, from the rounded hid
+    and da."""
     t = x.dtype
     x, nw, w1, b1, hid, da, dy = map(ref.wide, (x, nw, w1, b1, hid, da, dy))
     u, du = summed(hid, w1.t(), torch.zeros_like(hid), 1)
@@ -112,4 +112,5 @@ def norm_grads(x, nw, w1, b1, hid, da, dy, act, lo=True):
                   hat.abs() * (g * hat.abs()).mean(1, keepdim=True))
     return ((dx[0] + dy, dx[1] + off + E * (dx[0].abs() + dy.abs())),
             (dw[0], dw[1] + (ddh * hat.abs()).sum(0)),
-            (db[0], db[1] + ddh.sum(0)))
+            (db[0], db[1] + ddh.sum(0)),
+            (p.t() @ hid, summed(whole.t(), hid, dp.t(), 2)[1]))

@@ -39,5 +39,8 @@ def test_norm_gradients_of_the_block(t, act, rows, d, h):
     if rows < 100:
         assert outside(one[2][0], want[2]) > 0.1
         assert outside(one[1][0], want[1]) > 0.05
+        # of one row dw1 is a product that rounds once or twice
+        dw1 = one[3][0].to(t).double()
+        assert outside(dw1, want[3], t) > 0.02
     # one row has few values
     assert rows == 1 or outside(dx, want[0], t) > 0.02

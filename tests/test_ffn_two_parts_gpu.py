@@ -43,8 +43,10 @@ def test_norm_gradients_of_the_block(t, act, rows, d, h):
         a = gt.linear_act(hid, w1, b1, act=act)
     a.requires_grad_(True)
     da, = torch.autograd.grad(gt.linear_act(a, w2, b2, x), a, dy)
-    got = torch.autograd.grad(gt.ffn_block(*args, act=act), [x, nw, nb], dy)
+    got = torch.autograd.grad(gt.ffn_block(*args, act=act), [x, nw, nb, w1],
+                              dy)
     want = parts.norm_grads(x, nw, w1, b1, hid, da, dy, act)
     ref.close(got[2], *want[2], what="norm bias")
     ref.close(got[1], *want[1], what="norm weight")
     ref.close(got[0], *ref.rounded(*want[0], t), what="dx")
+    ref.close(got[3], *ref.rounded(*want[3], t), what="dw1")
