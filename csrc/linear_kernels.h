@@ -220,12 +220,12 @@ __device__ __forceinline__ void put_sum(const EpiArgs& e, long long m, int left,
 // tile's fp32 sums go to part[blockIdx.y][m][n] (rows of ld_part values), and
 // finish_kernel joins them; otherwise the epilogue follows at once.
 //
-// What the epilogues cost, 17920 x 10000 results in bf16, us of the whole kernel
-// at k = 64 and 1500: plain 123 and 588 (the results alone take 69 at a copy's
-// rate), forward with bias 139 and 602, with gelu too 228 and 695, and its input
-// kept 244 and 712, or kept in 8 bits 288 and 760; a residual 241 and 683; a
-// gradient through gelu from the kept input 344 and 743, from its 8 bits 323 and
-// 727.  Gelu and its slope are bound by the vector unit, the others by memory.
+// What the epilogues cost, 17920 x 10000 results in bf16, operands on lines, us of
+// the whole kernel at k = 64 and 1500: no bias 147 and 560 (the results alone take
+// 69 at a copy's rate), bias 151 and 565, with gelu too 253 and 657, and its input
+// kept 262 and 714, or kept in 8 bits 293 and 704; a residual 242 and 637; a
+// gradient through gelu from the kept input 355 and 770, from its 8 bits 328 and
+// 755.  Gelu and its slope are bound by the vector unit, the others by memory.
 template <typename T, int BM, int BN, int WM, int WN, bool AA, bool BA,
           int EPI>
 __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(
