@@ -17,25 +17,26 @@ def normal(*shape, seed=0):
     return torch.randn(*shape, generator=g).to(torch.bfloat16).to(DEV)
 
 
-X, W, B, R = normal(6, 40), normal(24, 40), normal(24), normal(6, 24)
-G, H = normal(40, seed=1), normal(40, seed=2)
-W2, B2 = normal(40, 24), normal(40, seed=3)
-# name, call, arguments
+# name, call, shapes of its arguments
 CALLS = {
-    "layer_norm": (gt.layer_norm, (X, G, H)),
+    "layer_norm": (gt.layer_norm, [(6, 40), (40,), (40,)]),
     "linear_act": (lambda x, w, b, r: gt.linear_act(x, w, b, r, act="gelu"),
-                   (X, W, B, R)),
-    "ffn_block": (gt.ffn_block, (X, G, H, W, B, W2, B2)),
+                   [(6, 40), (24, 40), (24,), (6, 24)]),
+    "ffn_block": (gt.ffn_block, [(6, 40), (40,), (40,), (24, 40), (24,),
+                                 (40, 24), (40,)]),
 }
 EVERY = [(name, i) for name, (_, args) in CALLS.items()
          for i in range(len(args))]
 
 
+def arguments(name):
+    return [normal(*s, seed=i) for i, s in enumerate(CALLS[name][1])]
+
+
 @pytest.mark.parametrize("name,i", EVERY)
 @pytest.mark.parametrize("grad", [False, True])
 def test_forward_mode_is_refused(name, i, grad):
-    call, args = CALLS[name]
-    args = [a.detach().clone() for a in args]
+    call, args = CALLS[name][0], arguments(name)
     with fwd.dual_level():
         args[i] = fwd.make_dual(args[i].requires_grad_(grad),
                                 torch.ones_like(args[i]))
@@ -62,10 +63,10 @@ def test_forward_mode_of_the_8_bit_form_is_refused():
 @pytest.mark.parametrize("grad", [False, True])
 def test_tracing_is_refused(name, grad):
     if name == "act8":
-        call, args = (lambda x: gt.act8_unpack(*gt.act8_pack(x))), (X,)
+        call, args = (lambda x: gt.act8_unpack(*gt.act8_pack(x))), [normal(6, 40)]
     else:
-        call, args = CALLS[name]
-    args = tuple(a.detach().clone().requires_grad_(grad) for a in args)
+        call, args = CALLS[name][0], arguments(name)
+    args = tuple(a.requires_grad_(grad) for a in args)
     with pytest.raises(RuntimeError, match="traced"):
         torch.jit.trace(call, args, check_trace=False)
     call(*args)
@@ -73,7 +74,7 @@ def test_tracing_is_refused(name, grad):
 
 @pytest.mark.parametrize("name", list(CALLS))
 def test_function_transforms_are_refused(name):
-    call, args = CALLS[name]
+    call, args = CALLS[name][0], arguments(name)
 
     def of_x(x):
         return call(x, *args[1:])
@@ -90,7 +91,7 @@ def test_function_transforms_are_refused(name):
 @pytest.mark.parametrize("mode", ["real", "fake"])
 def test_graphs_of_calls_are_refused(name, mode):
     from torch.fx.experimental.proxy_tensor import make_fx
-    call, args = CALLS[name]
+    call, args = CALLS[name][0], arguments(name)
     with pytest.raises(RuntimeError):
         make_fx(call, tracing_mode=mode)(*args)
 
@@ -98,8 +99,8 @@ def test_graphs_of_calls_are_refused(name, mode):
 @pytest.mark.parametrize("name", list(CALLS))
 def test_compiled_programs_call_them(name):
     """torch.compile leaves its graph for the call and goes on after it."""
-    call, args = CALLS[name]
-    args = [a.detach().clone().requires_grad_(True) for a in args]
+    call = CALLS[name][0]
+    args = [a.requires_grad_(True) for a in arguments(name)]
 
     def program(*a):
         return call(a[0] * 2, *a[1:]) + 1

@@ -1,15 +1,11 @@
 """The default name of a run, under which its checkpoints lie, tells runs of
 other models apart."""
-import os
-import subprocess
 import sys
 
 import pytest
+from torch import nn
 
-REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-ARGS = ["--dnn", "lstm", "--dataset", "ptb", "--device", "cpu", "--no-amp",
-        "--num-workers", "0", "--batch-size", "2", "--max-epochs", "1",
-        "--iters-per-epoch", "1", "--n-samples", "4"]
+from gtopkssgd_amd.checkpoint import latest_checkpoint, save_checkpoint
 
 
 def tag(monkeypatch, *extra):
@@ -34,10 +30,10 @@ def test_tag_without_the_block_is_as_before(monkeypatch):
 
 @pytest.mark.parametrize("first,then", [([], ["--ffn-mult", "1"]),
                                         (["--ffn-mult", "1"], [])])
-def test_resume_leaves_another_models_checkpoint(tmp_path, first, then):
-    for extra in (first, [*then, "--resume"]):
-        r = subprocess.run(
-            [sys.executable, os.path.join(REPO, "train.py"), *ARGS, *extra,
-             "--checkpoint-dir", str(tmp_path)],
-            cwd=REPO, capture_output=True, text=True, timeout=300)
-        assert r.returncode == 0, r.stderr[-2000:]
+def test_resume_leaves_another_models_checkpoint(tmp_path, monkeypatch, first,
+                                                 then):
+    base = ["--dnn", "lstm", "--dataset", "ptb"]
+    tags = [tag(monkeypatch, *base, *extra) for extra in (first, then)]
+    path = save_checkpoint(str(tmp_path), tags[0], 0, nn.Linear(2, 2))
+    assert latest_checkpoint(str(tmp_path), tags[0]) == path
+    assert latest_checkpoint(str(tmp_path), tags[1]) is None
